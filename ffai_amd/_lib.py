@@ -158,6 +158,11 @@ def load():
     L.ffai_vocab_int8_workspace_bytes.argtypes = [i32, i32, ctypes.POINTER(ctypes.c_size_t)]
     L.ffai_vocab_int8_logits.argtypes = [vp, vp, vp, i32, i32, i32, vp, i32, i64, vp, i64, vp,
                                          ctypes.c_size_t, vp]
+    lp = ctypes.POINTER(ctypes.c_int64)
+    L.ffai_prefix_attn_fwd.argtypes = [cp, cp, vp, i32, i32, i32, lp, ctypes.c_float, vp, i32, lp,
+                                       vp, sz, vp]
+    L.ffai_prefix_attn_workspace_bytes.argtypes = [cp, cp, i32, i32, ctypes.POINTER(sz)]
+    L.ffai_prefix_attn_plan_info.argtypes = [cp, cp, i32, i32, ip]
     L.ffai_probe_empty.argtypes = [ctypes.c_int, vp]
     L.ffai_probe_read.argtypes = [vp, sz, vp, ctypes.c_int, vp]
     L.ffai_probe_pipes.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, vp, vp]
@@ -172,7 +177,9 @@ def load():
                  "ffai_cross_kv_build", "ffai_encoder_attn_workspace_bytes",
                  "ffai_encoder_attn_fwd", "ffai_gemv_f16", "ffai_gemv_f16_plan_info",
                  "ffai_vocab_int8_quantize",
-                 "ffai_vocab_int8_workspace_bytes", "ffai_vocab_int8_logits"):
+                 "ffai_vocab_int8_workspace_bytes", "ffai_vocab_int8_logits",
+                 "ffai_prefix_attn_fwd", "ffai_prefix_attn_workspace_bytes",
+                 "ffai_prefix_attn_plan_info"):
         getattr(L, name).restype = ctypes.c_int
     _lib = L
     return L
@@ -231,6 +238,40 @@ def get_fwd_split_override() -> tuple:
     a, b = ctypes.c_int(), ctypes.c_int()
     load().ffai_get_fwd_split_override(ctypes.byref(a), ctypes.byref(b))
     return a.value, b.value
+
+
+class _Here:
+    """The context of a device that is the current one already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device):
+    """A context in which `device` (of a tensor) is the current one: library calls launch on the
+    current device. Free where it already is. (Operands of host memory: nothing to select; the
+    library refuses or the caller has checked.)"""
+    import torch
+
+    if device.type != "cuda":
+        raise ValueError(f"operands must be on a HIP device, not {device}")
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def current_stream(device) -> int:
+    """The raw handle of `device`'s current stream (no Stream object around it)."""
+    import torch
+
+    index = torch._C._cuda_getDevice() if device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def last_error() -> str:

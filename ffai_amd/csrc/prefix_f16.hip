@@ -1,0 +1,10 @@
+// f16 instantiations of the shared-prefix attention kernels.
+#include "prefix_attn.cuh"
+
+namespace ffai {
+
+hipError_t launch_prefix_f16(const PrefixParams& p, int head_dim, int parts, hipStream_t s) {
+  return launch_prefix_type<kF16>(p, head_dim, parts, s);
+}
+
+}  // namespace ffai

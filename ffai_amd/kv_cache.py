@@ -42,6 +42,22 @@ class KVCache:
         self.layers = layers
         self.slots, self.heads, self.capacity, self.head_dim = slots, heads, capacity, head_dim
 
+    @classmethod
+    def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor) -> "KVCache":
+        """A cache over tensors that are there already: k and v (slots, heads, capacity, head_dim)
+        of one type and the same strides (views of a larger allocation too), lens int32[slots],
+        all on one device. Nothing is copied."""
+        if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride():
+            raise ValueError("k and v must be (slots, heads, capacity, head_dim), alike in shape, "
+                             "type and strides")
+        if k.dtype not in _DT or k.stride(3) != 1:
+            raise ValueError("k and v must be f32, f16 or bf16 with head_dim contiguous")
+        if lens.dtype != torch.int32 or lens.shape != k.shape[:1] or not lens.is_contiguous():
+            raise ValueError("lens must be a contiguous int32 tensor of one length per slot")
+        if v.device != k.device or lens.device != k.device:
+            raise ValueError("k, v and lens must be on one device")
+        return cls(*k.shape, _views=(k, v, lens))
+
     def layer(self, l: int) -> "KVCache":
         assert self.layers is not None and 0 <= l < self.layers
         return KVCache(self.slots, self.heads, self.capacity, self.head_dim,

@@ -197,6 +197,18 @@ extern "C" {
                                   workspace: *mut c_void, workspace_bytes: usize,
                                   stream: *mut c_void) -> c_int;
 
+    // ---- include/ffai_prefix.h
+    pub fn ffai_prefix_attn_fwd(prefix: *const ffai_kv_cache, own: *const ffai_kv_cache,
+                                q: *const c_void, q_dtype: i32, heads_q: i32, q_len: i32,
+                                q_strides: *const i64, scale: f32, out: *mut c_void,
+                                out_dtype: i32, o_strides: *const i64, workspace: *mut c_void,
+                                workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ffai_prefix_attn_workspace_bytes(prefix: *const ffai_kv_cache,
+                                            own: *const ffai_kv_cache, heads_q: i32, q_len: i32,
+                                            bytes: *mut usize) -> c_int;
+    pub fn ffai_prefix_attn_plan_info(prefix: *const ffai_kv_cache, own: *const ffai_kv_cache,
+                                      heads_q: i32, q_len: i32, info: *mut i32) -> c_int;
+
     // ---- include/ffai_probe.h (diagnostics)
     pub fn ffai_probe_empty(workgroups: c_int, stream: *mut c_void) -> c_int;
     pub fn ffai_probe_read(src: *const c_void, bytes: usize, out: *mut f32, workgroups: c_int,

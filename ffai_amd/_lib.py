@@ -163,6 +163,12 @@ def load():
                                        vp, sz, vp]
     L.ffai_prefix_attn_workspace_bytes.argtypes = [cp, cp, i32, i32, ctypes.POINTER(sz)]
     L.ffai_prefix_attn_plan_info.argtypes = [cp, cp, i32, i32, ip]
+    L.ffai_int8_quantize_rows.argtypes = [vp, i32, i32, i32, i64, vp, i64, vp, vp]
+    L.ffai_int8_product.argtypes = [vp, i64, vp, i32, i32, vp, i64, vp, vp, i32, vp, i32, i64, vp]
+    L.ffai_int8_linear.argtypes = [vp, i32, i64, i32, i32, vp, i64, vp, vp, i32, vp, i32, i64, vp,
+                                   sz, vp]
+    L.ffai_int8_linear_workspace_bytes.argtypes = [i32, i32, ctypes.POINTER(sz)]
+    L.ffai_int8_plan_info.argtypes = [i32, i32, i32, ip]
     L.ffai_probe_empty.argtypes = [ctypes.c_int, vp]
     L.ffai_probe_read.argtypes = [vp, sz, vp, ctypes.c_int, vp]
     L.ffai_probe_pipes.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, vp, vp]
@@ -179,7 +185,8 @@ def load():
                  "ffai_vocab_int8_quantize",
                  "ffai_vocab_int8_workspace_bytes", "ffai_vocab_int8_logits",
                  "ffai_prefix_attn_fwd", "ffai_prefix_attn_workspace_bytes",
-                 "ffai_prefix_attn_plan_info"):
+                 "ffai_prefix_attn_plan_info", "ffai_int8_quantize_rows", "ffai_int8_product",
+                 "ffai_int8_linear", "ffai_int8_linear_workspace_bytes", "ffai_int8_plan_info"):
         getattr(L, name).restype = ctypes.c_int
     _lib = L
     return L

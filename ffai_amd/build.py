@@ -4,9 +4,9 @@ hipcc compiles the kernel instantiations (fwd_bf16.hip, fwd_f16.hip, fwd_f32.hip
 decode_f16.hip, decode_vec.hip),
 the decode-state kernels and their C ABI (kv_cache.hip), the decoder GEMVs (gemv.hip), the
 launch-floor probes (probe.hip), the launch dispatch (attn_launch.hip), the attention C ABI
-(attn_api.cpp), the encoder attention block around hipBLASLt (encoder_attn.cpp) and attention over
-a shared prefix (prefix_bf16.hip, prefix_f16.hip, prefix.hip) for gfx950 only, in parallel, then
-links them into one shared library. Packed-FP32 VALU instructions are disabled for all device
+(attn_api.cpp), the encoder attention block around hipBLASLt (encoder_attn.cpp), attention over a
+shared prefix (prefix_bf16.hip, prefix_f16.hip, prefix.hip) and the 8-bit linear layers (int8.hip)
+for gfx950 only, in parallel, then links them into one shared library. Packed-FP32 VALU instructions are disabled for all device
 code.
 """
 
@@ -27,7 +27,8 @@ SOURCES = [os.path.join(CSRC, n) for n in
            ("fwd_bf16.hip", "fwd_f16.hip", "fwd_f32.hip", "decode.hip", "decode_f16.hip",
             "decode_vec.hip",
             "kv_cache.hip", "gemv.hip", "probe.hip", "attn_launch.hip", "attn_api.cpp",
-            "encoder_attn.cpp", "prefix_bf16.hip", "prefix_f16.hip", "prefix.hip")]
+            "encoder_attn.cpp", "prefix_bf16.hip", "prefix_f16.hip", "prefix.hip",
+            "int8.hip")]
 LIBS = ["-L/opt/rocm/lib", "-lhipblaslt", "-Wl,-rpath,/opt/rocm/lib"]
 ARCH = "gfx950"
 

@@ -1,0 +1,508 @@
+// Linear layers in 8-bit integers (include/ffai_int8.h): the quantization of rows and the product
+// of quantized rows with weights on the int8 matrix instructions.
+#include "../../include/ffai_int8.h"
+
+#include <algorithm>
+
+#include "attn_common.cuh"
+
+namespace ffai {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kStep = 128;  // contraction elements (bytes) of a product step
+
+// ---- quantization ----------------------------------------------------------------------------
+// Two passes over a row that stays in registers: its largest magnitude, then the quotients. The
+// magnitude is taken on the bit patterns (sign cleared, as integers: the order of non-negative
+// floats, with NaN above infinity), so that a NaN becomes the scale. Divisions are IEEE f32: the
+// quotient's rounding decides which integer a value near a half goes to.
+__device__ __forceinline__ int quant1(float x, float s) {
+  const float r = __builtin_rintf(x / s);
+  // NaN (of a non-finite row) to 0: the clamps compare bits of ordinary numbers only
+  const bool nan = (__float_as_uint(r) & 0x7fffffffu) > 0x7f800000u;
+  return nan ? 0 : (int)fminf(fmaxf(r, -127.f), 127.f);
+}
+__device__ __forceinline__ uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, s));
+  return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const store_t<DT>* row, int k, int dim, float x[8]) {
+  if (k + 8 <= dim) {
+    const f32x4 a = ld4f<DT>(row + k), b = ld4f<DT>(row + k + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = a[e];
+      x[4 + e] = b[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = 0.f;
+      if (k + e < dim) {
+        if constexpr (DT == kF32) x[e] = row[k + e];
+        else x[e] = to_f32<DT>(row[k + e]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ u32x2 quant8(const float x[8], float s) {
+  u32x2 r = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e >> 2] |= ((uint32_t)quant1(x[e], s) & 0xffu) << (8 * (e & 3));
+  return r;
+}
+
+__device__ __forceinline__ float row_scale(uint32_t top) {
+  return top == 0 ? 1.f : __uint_as_float(top) / 127.f;
+}
+
+// WPR waves a row (1: a wave per row, four rows a workgroup; 4: the workgroup's four waves share
+// a row, for few rows); NC > 0: the row fits NC chunks of 8 elements a lane and stays in
+// registers; NC == 0: any length, read twice. Bound by reading x and writing q.
+template <int DT, int WPR, int NC>
+__global__ __launch_bounds__(256) void int8_quantize_kernel(const void* xv, int64_t xs, int rows,
+                                                            int dim, int8_t* q, int64_t qs,
+                                                            float* scale) {
+  __shared__ uint32_t tops[4];
+  const int wave = item_id() >> 6;
+  const int t = WPR == 1 ? item_id() & 63 : item_id();
+  const int row = WPR == 1 ? wg_id_x() * 4 + wave : wg_id_x();
+  if (row >= rows) return;  // the whole wave (WPR 1); never with WPR 4
+  const store_t<DT>* x = reinterpret_cast<const store_t<DT>*>(xv) + (int64_t)row * xs;
+  int8_t* qr = q + (int64_t)row * qs;
+  const int end = (dim + kStep - 1) / kStep * kStep;  // q is zero from dim to here
+  constexpr int SPAN = WPR * 64 * 8;
+  uint32_t top = 0;
+  float v[NC > 0 ? NC : 1][8];
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      load8<DT>(x, c * SPAN + 8 * t, dim, v[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, mag(v[c][e]));
+    }
+  } else {
+    for (int k = 8 * t; k < dim; k += SPAN) {
+      load8<DT>(x, k, dim, v[0]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, mag(v[0][e]));
+    }
+  }
+  top = wave_umax(top);
+  if constexpr (WPR == 4) {
+    if ((t & 63) == 0) tops[wave] = top;
+    __syncthreads();
+    top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+  }
+  const float s = row_scale(top);
+  if (t == 0) scale[row] = s;
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int k = c * SPAN + 8 * t;
+      if (k < end) *reinterpret_cast<u32x2*>(qr + k) = quant8(v[c], s);
+    }
+  } else {
+    for (int k = 8 * t; k < end; k += SPAN) {
+      load8<DT>(x, k, dim, v[0]);
+      *reinterpret_cast<u32x2*>(qr + k) = quant8(v[0], s);
+    }
+  }
+}
+
+template <int DT>
+void launch_quantize(const void* x, int64_t xs, int rows, int dim, int8_t* q, int64_t qs,
+                     float* scale, hipStream_t st) {
+  const int end = (dim + kStep - 1) / kStep * kStep;
+  auto go = [&](auto kernel, int wpr) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(wpr == 1 ? (rows + 3) / 4 : rows)), dim3(256), 0, st,
+                       x, xs, rows, dim, q, qs, scale);
+  };
+  // few rows: a row's loads over four waves shorten its latency
+  if (rows <= 1024) {
+    if (end <= 2048) go(int8_quantize_kernel<DT, 4, 1>, 4);
+    else if (end <= 4096) go(int8_quantize_kernel<DT, 4, 2>, 4);
+    else if (end <= 8192) go(int8_quantize_kernel<DT, 4, 4>, 4);
+    else go(int8_quantize_kernel<DT, 4, 0>, 4);
+  } else {
+    if (end <= 512) go(int8_quantize_kernel<DT, 1, 1>, 1);
+    else if (end <= 1024) go(int8_quantize_kernel<DT, 1, 2>, 1);
+    else if (end <= 2048) go(int8_quantize_kernel<DT, 1, 4>, 1);
+    else if (end <= 4096) go(int8_quantize_kernel<DT, 1, 8>, 1);
+    else if (end <= 8192) go(int8_quantize_kernel<DT, 1, 16>, 1);
+    else go(int8_quantize_kernel<DT, 1, 0>, 1);
+  }
+}
+
+// ---- product ---------------------------------------------------------------------------------
+struct Int8Params {
+  const int8_t* x;
+  int64_t xs;
+  const float* sx;
+  const int8_t* w;
+  int64_t ws;
+  const float* sw;
+  const float* bias;
+  void* y;
+  int64_t ys;
+  int32_t rows, out_dim;
+  int32_t steps;  // kStep-byte contraction steps
+  int32_t w_last;  // the last 16-byte chunk of a row of w
+  int32_t tx, tw;  // tiles over the rows of x and of w
+};
+
+// s_waitcnt vmcnt(N) lgkmcnt(0)
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70);
+}
+
+// One tile of BX rows of x by BW rows of w per workgroup, waves in a grid of GX by GW, on
+// v_mfma_i32_32x32x32_i8 (lane l: row l % 32, 16 bytes at 16 (l / 32) of the 32): the weights are
+// the A operand, so a lane's results are four consecutive outputs of one row of x. Steps of 128
+// bytes of the contraction arrive by DMA in a ring of STAGES buffers, rows unpadded with their eight
+// 16-byte chunks XOR-permuted by the row's low bits, so that the DMA's lanes read whole 128-byte
+// rows and eight lanes of a fragment read cover all banks. One barrier a step: it says that the
+// step's loads of every wave have landed and that every wave has read the buffer the next loads
+// overwrite. Rows past the operands' ends are clamped (their results are not stored); contraction
+// bytes past in_dim are zero in x, so whatever w's clamped chunk holds there counts for nothing.
+template <int BX, int BW, int GX, int GW, int STAGES, int OCC, int OUT>
+__global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8Params p) {
+  constexpr int NW = GX * GW;
+  constexpr int FX = BX / GX / 32, FW = BW / GW / 32;  // fragments of a wave
+  constexpr int BUF = (BX + BW) * kStep;
+  constexpr int PB = (BX + BW) / 8 / NW;  // 1 KB DMA blocks of a wave and step
+  static_assert((BX + BW) % (8 * NW) == 0, "whole blocks per wave");
+  static_assert(PB * (STAGES - 1) <= 63, "outstanding loads fit the counter");
+  extern __shared__ __attribute__((aligned(16))) int8_t int8_lds[];
+  const int lane = item_id() & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(item_id() >> 6);
+  const int gx = wave % GX, gw = wave / GX;
+
+  // Workgroups go to the eight XCDs in turn: each XCD takes a run of consecutive tiles, w fastest,
+  // so that its L2 serves a few row blocks of x against all of w.
+  const int n = p.tx * p.tw;
+  int tile = wg_id_x();
+  {
+    const int per = n / 8, more = n % 8, xcd = tile & 7, at = tile >> 3;
+    tile = xcd * per + min(xcd, more) + at;
+  }
+  const int x0 = tile / p.tw * BX, w0 = tile % p.tw * BW;
+
+  const char* xb = reinterpret_cast<const char*>(p.x + (int64_t)x0 * p.xs);
+  const char* wb = reinterpret_cast<const char*>(p.w + (int64_t)w0 * p.ws);
+  const int lr = lane >> 3;
+  const int chunk = 16 * ((lane & 7) ^ lr);
+  uint32_t off[PB];
+#pragma unroll
+  for (int b = 0; b < PB; ++b) {
+    const int r = (wave * PB + b) * 8 + lr;
+    off[b] = r < BW ? (uint32_t)min(r, p.out_dim - 1 - w0) * (uint32_t)p.ws
+                    : (uint32_t)min(r - BW, p.rows - 1 - x0) * (uint32_t)p.xs;
+  }
+  const uint32_t lds0 = lds_addr(int8_lds) + wave * PB * 1024;
+  auto issue = [&](int step, int buf) {
+    const uint32_t kx = (uint32_t)(step * kStep + chunk);
+    const uint32_t kw = min(kx, (uint32_t)p.w_last);
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      const bool of_w = (wave * PB + b) * 8 < BW;  // wave-uniform
+      lds_dma16_sbase(of_w ? wb : xb, off[b] + (of_w ? kw : kx), lds0 + buf * BUF + b * 1024);
+    }
+  };
+
+  i32x16 acc[FW][FX];
+#pragma unroll
+  for (int i = 0; i < FW; ++i)
+#pragma unroll
+    for (int j = 0; j < FX; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < p.steps) issue(s, s);
+  const int row = lane & 31, half = lane >> 5;
+  int buf = 0, nbuf = STAGES - 1;
+#pragma unroll 1
+  for (int step = 0; step < p.steps; ++step) {
+    asm volatile("" ::: "memory");
+    if (STAGES > 2 && step + STAGES - 2 < p.steps) wait_vm<PB*(STAGES - 2)>();
+    else wait_vm<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (step + STAGES - 1 < p.steps) issue(step + STAGES - 1, nbuf);
+    const int8_t* base = int8_lds + buf * BUF;
+    const int8_t* wl = base + (gw * FW * 32 + row) * kStep;
+    const int8_t* xl = base + (BW + gx * FX * 32 + row) * kStep;
+    // fragments of the next 32 bytes are read under the products of the current ones (the
+    // scheduling barriers keep the compiler from reading all of them first, which spills)
+    i32x4 a[2][FW], b[2][FX];
+    auto frags = [&](int ks, i32x4 (&fa)[FW], i32x4 (&fb)[FX]) {
+      const int c = 16 * ((2 * ks + half) ^ (row & 7));
+#pragma unroll
+      for (int i = 0; i < FW; ++i) fa[i] = *reinterpret_cast<const i32x4*>(wl + i * 32 * kStep + c);
+#pragma unroll
+      for (int j = 0; j < FX; ++j) fb[j] = *reinterpret_cast<const i32x4*>(xl + j * 32 * kStep + c);
+    };
+    frags(0, a[0], b[0]);
+#pragma unroll
+    for (int ks = 0; ks < kStep / 32; ++ks) {
+      if (ks + 1 < kStep / 32) frags(ks + 1, a[(ks + 1) & 1], b[(ks + 1) & 1]);
+#pragma unroll
+      for (int i = 0; i < FW; ++i)
+#pragma unroll
+        for (int j = 0; j < FX; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks & 1][i], b[ks & 1][j], acc[i][j],
+                                                            0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    buf = buf + 1 == STAGES ? 0 : buf + 1;
+    nbuf = nbuf + 1 == STAGES ? 0 : nbuf + 1;
+  }
+
+  // ---- D lane l, element 4 q + r: w row 8 q + 4 (l / 32) + r, x row l % 32
+  float sx[FX];
+  int mrow[FX];
+#pragma unroll
+  for (int j = 0; j < FX; ++j) {
+    mrow[j] = x0 + (gx * FX + j) * 32 + row;
+    sx[j] = p.sx[min(mrow[j], p.rows - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < FW; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int o = w0 + (gw * FW + i) * 32 + 8 * q + 4 * half;
+      float sw[4], bias[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int oc = min(o + r, p.out_dim - 1);
+        sw[r] = p.sw[oc];
+        bias[r] = p.bias ? p.bias[oc] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < FX; ++j) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float t = (float)acc[i][j][4 * q + r] * sx[j];
+          v[r] = p.bias ? __builtin_fmaf(t, sw[r], bias[r]) : t * sw[r];
+        }
+        if (mrow[j] >= p.rows) continue;
+        store_t<OUT>* y = reinterpret_cast<store_t<OUT>*>(p.y) + (int64_t)mrow[j] * p.ys + o;
+        if (o + 4 <= p.out_dim) {
+          st4<OUT>(y, v);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (o + r < p.out_dim) {
+              if constexpr (OUT == kF32) y[r] = v[r];
+              else y[r] = from_f32<OUT>(v[r]);
+            }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+struct Int8Tile {
+  int bx, bw, waves, stages;
+};
+constexpr Int8Tile kTiles[] = {{256, 256, 8, 2}, {128, 128, 4, 2}, {64, 64, 4, 4}};
+
+int int8_tile(int rows, int out_dim) {
+  for (int t = 0; t < 2; ++t) {
+    const int64_t n = (int64_t)((rows + kTiles[t].bx - 1) / kTiles[t].bx) *
+                      ((out_dim + kTiles[t].bw - 1) / kTiles[t].bw);
+    if (n >= 256) return t;
+  }
+  return 2;
+}
+
+template <int BX, int BW, int GX, int GW, int STAGES, int OCC, int OUT>
+hipError_t launch_tile(const Int8Params& p, hipStream_t st) {
+  constexpr int lds = (BX + BW) * kStep * STAGES;
+  auto kernel = int8_product_kernel<BX, BW, GX, GW, STAGES, OCC, OUT>;
+  static const hipError_t once = hipFuncSetAttribute(
+      reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (once != hipSuccess) return once;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tx * p.tw)), dim3(GX * GW * 64), lds, st, p);
+  return hipGetLastError();
+}
+
+template <int OUT>
+hipError_t launch_product(Int8Params p, hipStream_t st) {
+  const int t = int8_tile(p.rows, p.out_dim);
+  p.tx = (p.rows + kTiles[t].bx - 1) / kTiles[t].bx;
+  p.tw = (p.out_dim + kTiles[t].bw - 1) / kTiles[t].bw;
+  if (t == 0) return launch_tile<256, 256, 2, 4, 2, 2, OUT>(p, st);
+  if (t == 1) return launch_tile<128, 128, 2, 2, 2, 2, OUT>(p, st);
+  return launch_tile<64, 64, 2, 2, 4, 2, OUT>(p, st);
+}
+
+bool known_dtype(int32_t d) { return d == FFAI_F32 || d == FFAI_F16 || d == FFAI_BF16; }
+size_t esize(int32_t d) { return d == FFAI_F32 ? 4 : 2; }
+constexpr int kMaxIn = 131072;  // 127 * 127 * in_dim stays below 2^31
+
+int check_dims(int32_t rows, int32_t in_dim) {
+  if (rows < 0) return api_fail(FFAI_ERR_INVALID, "rows must be >= 0");
+  if (in_dim < 1 || in_dim > kMaxIn) return api_fail(FFAI_ERR_INVALID, "in_dim must be in [1, 131072]");
+  return FFAI_OK;
+}
+int check_rows_of_x(const void* x, int32_t dt, int32_t rows, int32_t dim, int64_t xs) {
+  const int rc = check_dims(rows, dim);
+  if (rc != FFAI_OK) return rc;
+  if (!known_dtype(dt)) return api_fail(FFAI_ERR_INVALID, "unknown x dtype");
+  if (rows == 0) return FFAI_OK;
+  if (!x) return api_fail(FFAI_ERR_INVALID, "null x");
+  if ((uintptr_t)x % esize(dt)) return api_fail(FFAI_ERR_INVALID, "x must be aligned to its element size");
+  if (xs < 0 || (rows > 1 && xs < dim)) return api_fail(FFAI_ERR_INVALID, "x rows overlap");
+  return FFAI_OK;
+}
+int check_weights(const int8_t* w, int64_t ws, const float* sw, const float* bias, int32_t out_dim,
+                  int32_t in_dim, const void* y, int32_t y_dtype, int64_t ys, int32_t rows) {
+  if (!w || !sw || (rows > 0 && !y)) return api_fail(FFAI_ERR_INVALID, "null pointer");
+  if (out_dim < 1 || out_dim > (1 << 28)) return api_fail(FFAI_ERR_INVALID, "out_dim must be in [1, 2^28]");
+  if ((uintptr_t)w % 16 || ws % 16 || ws < in_dim || ws > (1 << 22))
+    return api_fail(FFAI_ERR_INVALID, "w must be 16-byte aligned with a row stride that is a multiple of 16 in [in_dim, 2^22]");
+  if ((uintptr_t)sw % 4 || (uintptr_t)bias % 4) return api_fail(FFAI_ERR_INVALID, "w_scale and bias must be 4-byte aligned");
+  if (!known_dtype(y_dtype)) return api_fail(FFAI_ERR_INVALID, "unknown y dtype");
+  if ((uintptr_t)y % esize(y_dtype)) return api_fail(FFAI_ERR_INVALID, "y must be aligned to its element size");
+  if (ys < 0 || (rows > 1 && ys < out_dim)) return api_fail(FFAI_ERR_INVALID, "y rows overlap");
+  if ((int64_t)((rows + 63) / 64) * ((out_dim + 63) / 64) > 0x7fffffff)
+    return api_fail(FFAI_ERR_INVALID, "problem too large");
+  return FFAI_OK;
+}
+
+hipError_t quantize(const void* x, int32_t dt, int32_t rows, int32_t dim, int64_t xs, int8_t* q,
+                    int64_t qs, float* scale, hipStream_t st) {
+  if (dt == FFAI_F32) launch_quantize<kF32>(x, xs, rows, dim, q, qs, scale, st);
+  else if (dt == FFAI_F16) launch_quantize<kF16>(x, xs, rows, dim, q, qs, scale, st);
+  else launch_quantize<kBF16>(x, xs, rows, dim, q, qs, scale, st);
+  return hipGetLastError();
+}
+
+hipError_t product(const int8_t* q, int64_t qs, const float* sx, int32_t rows, int32_t in_dim,
+                   const int8_t* w, int64_t ws, const float* sw, const float* bias,
+                   int32_t out_dim, void* y, int32_t y_dtype, int64_t ys, hipStream_t st) {
+  Int8Params p{};
+  p.x = q; p.xs = qs; p.sx = sx; p.w = w; p.ws = ws; p.sw = sw; p.bias = bias;
+  p.y = y; p.ys = ys; p.rows = rows; p.out_dim = out_dim;
+  p.steps = (in_dim + kStep - 1) / kStep;
+  p.w_last = (in_dim + 15) / 16 * 16 - 16;
+  return y_dtype == FFAI_F32   ? launch_product<kF32>(p, st)
+         : y_dtype == FFAI_F16 ? launch_product<kF16>(p, st)
+                               : launch_product<kBF16>(p, st);
+}
+
+int64_t row_bytes(int32_t dim) { return ((int64_t)dim + kStep - 1) / kStep * kStep; }
+
+}  // namespace
+}  // namespace ffai
+
+using namespace ffai;
+
+extern "C" {
+
+int ffai_int8_quantize_rows(const void* x, int32_t x_dtype, int32_t rows, int32_t dim,
+                            int64_t x_row_stride, int8_t* q, int64_t q_row_stride, float* scale,
+                            void* stream) {
+  api_clear_error();
+  int rc = check_rows_of_x(x, x_dtype, rows, dim, x_row_stride);
+  if (rc != FFAI_OK) return rc;
+  if (rows == 0) return FFAI_OK;
+  if (!q || !scale) return api_fail(FFAI_ERR_INVALID, "null pointer");
+  if ((uintptr_t)q % 16 || q_row_stride % kStep || q_row_stride < dim || q_row_stride > (1 << 22))
+    return api_fail(FFAI_ERR_INVALID, "q must be 16-byte aligned with a row stride that is a multiple of 128 in [dim, 2^22]");
+  if ((uintptr_t)scale % 4) return api_fail(FFAI_ERR_INVALID, "scale must be 4-byte aligned");
+  rc = api_check_device();
+  if (rc != FFAI_OK) return rc;
+  const hipError_t e = quantize(x, x_dtype, rows, dim, x_row_stride, q, q_row_stride, scale,
+                                static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));
+  return FFAI_OK;
+}
+
+int ffai_int8_product(const int8_t* q, int64_t q_row_stride, const float* scale, int32_t rows,
+                      int32_t in_dim, const int8_t* w, int64_t w_row_stride, const float* w_scale,
+                      const float* bias, int32_t out_dim, void* y, int32_t y_dtype,
+                      int64_t y_row_stride, void* stream) {
+  api_clear_error();
+  int rc = check_dims(rows, in_dim);
+  if (rc != FFAI_OK) return rc;
+  rc = check_weights(w, w_row_stride, w_scale, bias, out_dim, in_dim, y, y_dtype, y_row_stride, rows);
+  if (rc != FFAI_OK) return rc;
+  if (rows == 0) return FFAI_OK;
+  if (!q || !scale) return api_fail(FFAI_ERR_INVALID, "null pointer");
+  if ((uintptr_t)q % 16 || q_row_stride % kStep || q_row_stride < in_dim || q_row_stride > (1 << 22))
+    return api_fail(FFAI_ERR_INVALID, "q must be 16-byte aligned with a row stride that is a multiple of 128 in [in_dim, 2^22]");
+  if ((uintptr_t)scale % 4) return api_fail(FFAI_ERR_INVALID, "scale must be 4-byte aligned");
+  rc = api_check_device();
+  if (rc != FFAI_OK) return rc;
+  const hipError_t e = product(q, q_row_stride, scale, rows, in_dim, w, w_row_stride, w_scale, bias,
+                               out_dim, y, y_dtype, y_row_stride, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));
+  return FFAI_OK;
+}
+
+int ffai_int8_linear_workspace_bytes(int32_t rows, int32_t in_dim, size_t* bytes) {
+  api_clear_error();
+  if (!bytes) return api_fail(FFAI_ERR_INVALID, "null bytes pointer");
+  const int rc = check_dims(rows, in_dim);
+  if (rc != FFAI_OK) return rc;
+  *bytes = (size_t)rows * row_bytes(in_dim) + (((size_t)rows * 4 + 15) & ~size_t(15));
+  return FFAI_OK;
+}
+
+int ffai_int8_linear(const void* x, int32_t x_dtype, int64_t x_row_stride, int32_t rows,
+                     int32_t in_dim, const int8_t* w, int64_t w_row_stride, const float* w_scale,
+                     const float* bias, int32_t out_dim, void* y, int32_t y_dtype,
+                     int64_t y_row_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  api_clear_error();
+  int rc = check_rows_of_x(x, x_dtype, rows, in_dim, x_row_stride);
+  if (rc != FFAI_OK) return rc;
+  rc = check_weights(w, w_row_stride, w_scale, bias, out_dim, in_dim, y, y_dtype, y_row_stride, rows);
+  if (rc != FFAI_OK) return rc;
+  if (rows == 0) return FFAI_OK;
+  size_t need = 0;
+  ffai_int8_linear_workspace_bytes(rows, in_dim, &need);
+  if (!workspace || workspace_bytes < need)
+    return api_fail(FFAI_ERR_WORKSPACE, "workspace smaller than ffai_int8_linear_workspace_bytes");
+  if ((uintptr_t)workspace % 16) return api_fail(FFAI_ERR_INVALID, "workspace must be 16-byte aligned");
+  rc = api_check_device();
+  if (rc != FFAI_OK) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int8_t* q = static_cast<int8_t*>(workspace);
+  float* sx = reinterpret_cast<float*>(q + (size_t)rows * row_bytes(in_dim));
+  hipError_t e = quantize(x, x_dtype, rows, in_dim, x_row_stride, q, row_bytes(in_dim), sx, st);
+  if (e == hipSuccess)
+    e = product(q, row_bytes(in_dim), sx, rows, in_dim, w, w_row_stride, w_scale, bias, out_dim, y,
+                y_dtype, y_row_stride, st);
+  if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));
+  return FFAI_OK;
+}
+
+int ffai_int8_plan_info(int32_t rows, int32_t in_dim, int32_t out_dim, int32_t* info) {
+  api_clear_error();
+  if (!info) return api_fail(FFAI_ERR_INVALID, "null info pointer");
+  const int rc = check_dims(rows, in_dim);
+  if (rc != FFAI_OK) return rc;
+  if (rows < 1 || out_dim < 1 || out_dim > (1 << 28)) return api_fail(FFAI_ERR_INVALID, "rows >= 1 and out_dim in [1, 2^28]");
+  const Int8Tile t = kTiles[int8_tile(rows, out_dim)];
+  info[0] = t.bx;
+  info[1] = t.bw;
+  info[2] = t.waves;
+  info[3] = ((rows + t.bx - 1) / t.bx) * ((out_dim + t.bw - 1) / t.bw);
+  return FFAI_OK;
+}
+
+}  // extern "C"

@@ -209,6 +209,22 @@ extern "C" {
     pub fn ffai_prefix_attn_plan_info(prefix: *const ffai_kv_cache, own: *const ffai_kv_cache,
                                       heads_q: i32, q_len: i32, info: *mut i32) -> c_int;
 
+    // ---- include/ffai_int8.h
+    pub fn ffai_int8_quantize_rows(x: *const c_void, x_dtype: i32, rows: i32, dim: i32,
+                                   x_row_stride: i64, q: *mut i8, q_row_stride: i64,
+                                   scale: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ffai_int8_product(q: *const i8, q_row_stride: i64, scale: *const f32, rows: i32,
+                             in_dim: i32, w: *const i8, w_row_stride: i64, w_scale: *const f32,
+                             bias: *const f32, out_dim: i32, y: *mut c_void, y_dtype: i32,
+                             y_row_stride: i64, stream: *mut c_void) -> c_int;
+    pub fn ffai_int8_linear(x: *const c_void, x_dtype: i32, x_row_stride: i64, rows: i32,
+                            in_dim: i32, w: *const i8, w_row_stride: i64, w_scale: *const f32,
+                            bias: *const f32, out_dim: i32, y: *mut c_void, y_dtype: i32,
+                            y_row_stride: i64, workspace: *mut c_void, workspace_bytes: usize,
+                            stream: *mut c_void) -> c_int;
+    pub fn ffai_int8_linear_workspace_bytes(rows: i32, in_dim: i32, bytes: *mut usize) -> c_int;
+    pub fn ffai_int8_plan_info(rows: i32, in_dim: i32, out_dim: i32, info: *mut i32) -> c_int;
+
     // ---- include/ffai_probe.h (diagnostics)
     pub fn ffai_probe_empty(workgroups: c_int, stream: *mut c_void) -> c_int;
     pub fn ffai_probe_read(src: *const c_void, bytes: usize, out: *mut f32, workgroups: c_int,

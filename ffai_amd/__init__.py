@@ -11,9 +11,10 @@ The product is ``libffai_attn.so`` (C ABI: ``include/ffai_*.h``); this package b
   kernel);
 * ``ffai_amd.gemv``: the decoder's single-row projections and the int8 vocabulary head;
 * ``ffai_amd.prefix``: attention of many slots over a prefix they share and their own keys;
-* ``ffai_amd.int8``: linear layers in 8-bit integers, any number of rows.
+* ``ffai_amd.int8``: linear layers in 8-bit integers, any number of rows;
+* ``ffai_amd.sampling``: a token per row of logits: temperature, top-k, min-p and top-p.
 """
 
 from . import _lib  # noqa: F401
 
-__all__ = ["flash_attn", "kv_cache", "encoder", "gemv", "prefix", "int8", "build"]
+__all__ = ["flash_attn", "kv_cache", "encoder", "gemv", "prefix", "int8", "sampling", "build"]

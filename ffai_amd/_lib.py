@@ -169,6 +169,10 @@ def load():
                                    sz, vp]
     L.ffai_int8_linear_workspace_bytes.argtypes = [i32, i32, ctypes.POINTER(sz)]
     L.ffai_int8_plan_info.argtypes = [i32, i32, i32, ip]
+    f32 = ctypes.c_float
+    L.ffai_sample.argtypes = [vp, i32, i32, i32, i64, vp, f32, vp, i32, vp, f32, vp, f32, vp, vp,
+                              vp, vp, sz, vp]
+    L.ffai_sample_workspace_bytes.argtypes = [i32, i32, ctypes.POINTER(sz)]
     L.ffai_probe_empty.argtypes = [ctypes.c_int, vp]
     L.ffai_probe_read.argtypes = [vp, sz, vp, ctypes.c_int, vp]
     L.ffai_probe_pipes.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, vp, vp]
@@ -186,7 +190,8 @@ def load():
                  "ffai_vocab_int8_workspace_bytes", "ffai_vocab_int8_logits",
                  "ffai_prefix_attn_fwd", "ffai_prefix_attn_workspace_bytes",
                  "ffai_prefix_attn_plan_info", "ffai_int8_quantize_rows", "ffai_int8_product",
-                 "ffai_int8_linear", "ffai_int8_linear_workspace_bytes", "ffai_int8_plan_info"):
+                 "ffai_int8_linear", "ffai_int8_linear_workspace_bytes", "ffai_int8_plan_info",
+                 "ffai_sample", "ffai_sample_workspace_bytes"):
         getattr(L, name).restype = ctypes.c_int
     _lib = L
     return L

@@ -5,8 +5,8 @@ decode_f16.hip, decode_vec.hip),
 the decode-state kernels and their C ABI (kv_cache.hip), the decoder GEMVs (gemv.hip), the
 launch-floor probes (probe.hip), the launch dispatch (attn_launch.hip), the attention C ABI
 (attn_api.cpp), the encoder attention block around hipBLASLt (encoder_attn.cpp), attention over a
-shared prefix (prefix_bf16.hip, prefix_f16.hip, prefix.hip) and the 8-bit linear layers (int8.hip)
-for gfx950 only, in parallel, then links them into one shared library. Packed-FP32 VALU instructions are disabled for all device
+shared prefix (prefix_bf16.hip, prefix_f16.hip, prefix.hip), the 8-bit linear layers (int8.hip) and
+sampling (sample.hip) for gfx950 only, in parallel, then links them into one shared library. Packed-FP32 VALU instructions are disabled for all device
 code.
 """
 
@@ -28,7 +28,7 @@ SOURCES = [os.path.join(CSRC, n) for n in
             "decode_vec.hip",
             "kv_cache.hip", "gemv.hip", "probe.hip", "attn_launch.hip", "attn_api.cpp",
             "encoder_attn.cpp", "prefix_bf16.hip", "prefix_f16.hip", "prefix.hip",
-            "int8.hip")]
+            "int8.hip", "sample.hip")]
 LIBS = ["-L/opt/rocm/lib", "-lhipblaslt", "-Wl,-rpath,/opt/rocm/lib"]
 ARCH = "gfx950"
 

@@ -6,11 +6,11 @@
 use std::path::{Path, PathBuf};
 use std::process::Command;
 
-const SOURCES: [&str; 16] = [
+const SOURCES: [&str; 17] = [
     "fwd_bf16.hip", "fwd_f16.hip", "fwd_f32.hip", "decode.hip", "decode_f16.hip", "decode_vec.hip",
     "kv_cache.hip",
     "gemv.hip", "probe.hip", "attn_launch.hip", "attn_api.cpp", "encoder_attn.cpp",
-    "prefix_bf16.hip", "prefix_f16.hip", "prefix.hip", "int8.hip",
+    "prefix_bf16.hip", "prefix_f16.hip", "prefix.hip", "int8.hip", "sample.hip",
 ];
 
 fn hipcc() -> PathBuf {

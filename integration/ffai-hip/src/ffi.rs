@@ -225,6 +225,15 @@ extern "C" {
     pub fn ffai_int8_linear_workspace_bytes(rows: i32, in_dim: i32, bytes: *mut usize) -> c_int;
     pub fn ffai_int8_plan_info(rows: i32, in_dim: i32, out_dim: i32, info: *mut i32) -> c_int;
 
+    // ---- include/ffai_sample.h
+    pub fn ffai_sample(logits: *const c_void, logits_dtype: i32, rows: i32, vocab: i32,
+                       logits_row_stride: i64, temperature: *const f32, temperature_all: f32,
+                       top_k: *const i32, top_k_all: i32, top_p: *const f32, top_p_all: f32,
+                       min_p: *const f32, min_p_all: f32, u: *const f32, tokens: *mut i32,
+                       logprobs: *mut f32, workspace: *mut c_void, workspace_bytes: usize,
+                       stream: *mut c_void) -> c_int;
+    pub fn ffai_sample_workspace_bytes(rows: i32, vocab: i32, bytes: *mut usize) -> c_int;
+
     // ---- include/ffai_probe.h (diagnostics)
     pub fn ffai_probe_empty(workgroups: c_int, stream: *mut c_void) -> c_int;
     pub fn ffai_probe_read(src: *const c_void, bytes: usize, out: *mut f32, workgroups: c_int,

@@ -1,18 +1,22 @@
 // Sampling of one token per row of logits (include/ffai_sample.h).
 //
-// Two launches. sample_scan_kernel reads the logits once, spread over the whole GPU: per chunk of
-// a row its maximum and weight sums, per 1024 elements their maximum. sample_pick_kernel, one
-// workgroup a row, joins them and finds the token:
-//   * no filter: the chunk that holds u W by a scan of the chunks' sums, then the token in it;
-//   * filters: nearly always few tokens can be kept. The k-th largest of the 1024-element maxima
-//     bounds the k-th largest logit from below, so one pass collects everything from there up
-//     (k + a few tokens) in LDS, where it is sorted and the definition is applied as it stands;
-//   * otherwise (thousands of tokens kept, many equal ones): the boundary is found by histograms
-//     of counts or weights, finer each time, down to a list or a single value.
+// Two launches, three where a row may filter:
+//   * sample_scan_kernel reads the logits, spread over the whole GPU: of every 1024 elements (a
+//     wave's) the maximum, those of its four rows of lanes, and the weights' sum;
+//   * sample_gather_kernel: nearly always few tokens can be kept. The k-th largest group maximum
+//     bounds the k-th largest logit from below, so a second spread pass lists everything from there
+//     up (k and a few tokens more);
+//   * sample_pick_kernel, one workgroup a row, finds the token. No filter: the group that holds
+//     u W by a scan of the groups' sums, then the token in it, an element a thread.
+//     Filters: the list is ordered in LDS and the definition applied as it stands. Where it does
+//     not hold all that can be kept (thousands of tokens, many equal ones) the workgroup finds the
+//     boundary by histograms of counts or weights over the row, finer each time, down to a list or
+//     a single value.
 // Weights are 64-bit throughout: a token's share may be 1e-5 of the row's, and with f32 sums the
 // token at a given u would depend on the order of summation. f64 FMAs run at the f32 rate here;
-// an exponential is 20 of them. Histogram weights alone are integers (2^-43 steps: adding them in
-// any order gives the same sum), and what they decide is confirmed with f64 sums.
+// an exponential is 18 instructions. Only a histogram's weights are less (integers of f32
+// exponentials: adding them in any order gives the same sum), and what they decide is confirmed
+// with f64 sums.
 #include "../../include/ffai_sample.h"
 
 #include <algorithm>
@@ -22,18 +26,20 @@
 namespace ffai {
 namespace {
 
-constexpr int kChunk = 4096;  // elements of a scan workgroup
-constexpr int kGroup = 1024;  // elements of one of its waves
+constexpr int kGroup = 1024;  // elements whose maximum and sums a scan wave leaves
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kPick = 1024;  // threads of a pick workgroup
-constexpr int kList = 2048;  // tokens of an LDS list
-constexpr int kBins = 2048;
-constexpr int kSegs = 4096;  // ordered segments of a row at most (kMaxVocab / (64 * 4))
+constexpr int kPick = 1024;   // threads of a pick workgroup
+constexpr int kWaves = kPick / 64;
+constexpr int kShort = 256;   // tokens of a list that one wave finishes
+constexpr int kList = 2048;   // tokens of an LDS list
+constexpr int kBins = 4096;
+constexpr int kChunk = 4096;  // elements of a gather workgroup's share
+constexpr int kAhead = 4;     // steps of a pass over a row that a wave loads ahead
 
 struct SampleParams {
   const void* logits;
   int64_t ls;
-  int32_t rows, vocab, chunks;
+  int32_t rows, vocab, groups, chunks;
   const float* t;
   const int32_t* k;
   const float* p;
@@ -43,10 +49,13 @@ struct SampleParams {
   const float* u;
   int32_t* tok;
   float* lp;
-  double* sum_t;   // [row][chunk] sum of exp((l - chunk max) / T)
-  double* sum_1;   // [row][chunk] sum of exp(l - chunk max)
-  float* gmax;     // [row][chunk * 4 + wave] maxima
-  int32_t* first;  // [row][chunk] index of the chunk's first maximum
+  double* sum_t;   // [row][group] sum of exp((l - group max) / T)
+  double* sum_1;   // [row][group] sum of exp(l - group max)
+  float* gmax;     // [row][group] maxima
+  float* smax;     // [row][group][4] of the group's four rows of lanes
+  float* low;      // [row] the least logit that is listed; -inf: no list
+  int32_t* count;  // [row][chunk] listed tokens (kShort at most are held)
+  uint64_t* cand;  // [row][chunk][kShort] their ranks, in no order
 };
 
 // The device code is compiled for numbers that are not NaN, so NaN is recognised by its bits, and
@@ -60,20 +69,24 @@ __device__ __forceinline__ float nan_to_low(float x) {
   return r;
 }
 
+constexpr double kLog2e = 1.4426950408889634074;
+
 struct RowSettings {
   bool greedy;
-  double inv;  // 1 / T
-  int k;       // 0: off
-  float p;     // 1: off
-  double mp;   // 0: off
-  __device__ bool filtered() const { return k > 0 || p < 1.f || mp > 0.0; }
+  double inv2;  // log2(e) / T
+  bool t1;      // T is 1
+  int k;        // 0: off
+  float p;      // 1: off
+  double mp;    // 0: off
+  __device__ __forceinline__ bool filtered() const { return k > 0 || p < 1.f || mp > 0.0; }
 };
 __device__ __forceinline__ RowSettings settings(const SampleParams& p, int row) {
   RowSettings s;
   const float t = p.t ? p.t[row] : p.t_all;
   const uint32_t tb = __float_as_uint(t);
   s.greedy = !(tb > 0u && tb <= 0x7f800000u);  // positive, infinity included
-  s.inv = 1.0 / (double)t;
+  s.inv2 = __builtin_fmax(kLog2e / (double)t, 1e-300);  // (T = inf: -inf times it stays -inf)
+  s.t1 = t == 1.f;
   const int k = p.k ? p.k[row] : p.k_all;
   s.k = k <= 0 || k >= p.vocab ? 0 : k;
   const float tp = p.p ? p.p[row] : p.p_all;
@@ -83,35 +96,44 @@ __device__ __forceinline__ RowSettings settings(const SampleParams& p, int row) 
   return s;
 }
 
-// exp(z), z <= 0: z = n ln 2 + r, |r| <= ln 2 / 2, by two-part reduction, exp(r) by its Taylor sum
-// to r^13 / 13! (the next term is below 2^-58), times 2^n.
-__device__ __forceinline__ double exp_neg(double z) {
-  if (z < -745.0) return 0.0;
-  const double n = __builtin_rint(z * 1.4426950408889634074);
-  double r = __builtin_fma(-n, 0x1.62e42fefa3800p-1, z);  // ln 2, its leading 42 bits
-  r = __builtin_fma(-n, 0x1.ef35793c76730p-45, r);        // and the rest
-  double e = 1.0 / 6227020800.0;
-  e = __builtin_fma(e, r, 1.0 / 479001600.0);
-  e = __builtin_fma(e, r, 1.0 / 39916800.0);
-  e = __builtin_fma(e, r, 1.0 / 3628800.0);
-  e = __builtin_fma(e, r, 1.0 / 362880.0);
-  e = __builtin_fma(e, r, 1.0 / 40320.0);
-  e = __builtin_fma(e, r, 1.0 / 5040.0);
-  e = __builtin_fma(e, r, 1.0 / 720.0);
-  e = __builtin_fma(e, r, 1.0 / 120.0);
-  e = __builtin_fma(e, r, 1.0 / 24.0);
-  e = __builtin_fma(e, r, 1.0 / 6.0);
-  e = __builtin_fma(e, r, 0.5);
-  e = __builtin_fma(e, r, 1.0);
-  e = __builtin_fma(e, r, 1.0);
-  return __builtin_ldexp(e, (int)n);
+// a b + c with c in scalar registers: one instruction. (The compiler's choice is an accumulating
+// form that first copies c to vector registers, two instructions a term.)
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
 }
-// A token's weight against the largest logit m. (l < m strictly below: 1 at m even where both
-// are infinite.)
-__device__ __forceinline__ double weight(float l, float m, double inv) {
-  if (l >= m) return l == kNegInf ? 0.0 : 1.0;
-  if (l == kNegInf || m == __builtin_inff()) return 0.0;
-  return exp_neg(((double)l - (double)m) * inv);
+// 2^y, y <= 0 (0 below -1000): 2^n times 2^f, n the whole number nearest to y, |f| <= 1/2 by the
+// polynomial of degree 10 that equals it at the Chebyshev points (relative error below 3e-16; exactly
+// 1 at 0). n comes as the low bits of y + 1.5 2^52, and goes into the exponent field: additions and
+// FMAs, which run at the f32 rate. A weight's exponent carries the rounding of its own product,
+// about |y| 2^-53: 1e-14 at most where it counts.
+__device__ __forceinline__ double exp2_neg(double y) {
+  constexpr double kMagic = 0x1.8p52;
+  const double t = y + kMagic;
+  const double f = y - (t - kMagic);
+  double e = 0x1.e6063f7217bc6p-28;
+  e = fma_const(e, f, 0x1.b675bca4eeebbp-24);
+  e = fma_const(e, f, 0x1.62bfd47773353p-20);
+  e = fma_const(e, f, 0x1.ffcb54062e698p-17);
+  e = fma_const(e, f, 0x1.430913096fd9fp-13);
+  e = fma_const(e, f, 0x1.5d87fe9d7a584p-10);
+  e = fma_const(e, f, 0x1.3b2ab6fba1ddap-7);
+  e = fma_const(e, f, 0x1.c6b08d703ce49p-5);
+  e = fma_const(e, f, 0x1.ebfbdff82c598p-3);
+  e = fma_const(e, f, 0x1.62e42fefa3a19p-1);
+  e = __builtin_fma(e, f, 1.0);
+  const uint64_t eb = __builtin_bit_cast(uint64_t, e), tb = __builtin_bit_cast(uint64_t, t);
+  const uint32_t hi = (uint32_t)(eb >> 32) + ((uint32_t)tb << 20);
+  // (negative numbers: the larger the bits, the lower the number; -inf too)
+  const bool under = (uint32_t)(__builtin_bit_cast(uint64_t, y) >> 32) > 0xc08f4000u;
+  const uint64_t r = ((uint64_t)(under ? 0u : hi) << 32) | (under ? 0u : (uint32_t)eb);
+  return __builtin_bit_cast(double, r);
+}
+// A token's weight against the largest logit m (l <= m): 1 at m even where both are infinite.
+__device__ __forceinline__ double weight(float l, float m, double inv2) {
+  if (m == __builtin_inff()) return l >= m ? 1.0 : 0.0;  // uniform
+  return exp2_neg(((double)l - (double)m) * inv2);
 }
 
 template <int DT>
@@ -119,27 +141,60 @@ __device__ __forceinline__ float load1(const store_t<DT>* x, int i) {
   if constexpr (DT == kF32) return nan_to_low(x[i]);
   else return nan_to_low(to_f32<DT>(x[i]));
 }
-// EPL consecutive logits from index i; -inf past the row's end.
-template <int DT>
+// EPL consecutive logits from index i of a row of n (TINY: n < EPL); -inf from index `end` on. Loads
+// have no branch: the address is clamped into the row, and a step that reaches past `end` puts its
+// elements right afterwards (`fix`). A load on one side of a branch makes the compiler wait for all
+// loads at the join: a pass over a row then had one step's loads in flight, 1.2 us a step.
+template <int DT, bool TINY>
 struct Lane {
   static constexpr int EPL = DT == kF32 ? 4 : 8;
+  using S = store_t<DT>;
   float v[EPL];
-  __device__ __forceinline__ void load(const store_t<DT>* x, int i, int n) {
-    if (i + EPL <= n) {
-      if constexpr (DT == kF32) {
-        const f32x4 a = *reinterpret_cast<const f32x4_e*>(x + i);
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) v[e] = nan_to_low(a[e]);
-      } else {
-        const u32x4 a = ld16h(x + i);
-#pragma unroll
-        for (int e = 0; e < EPL; ++e)
-          v[e] = nan_to_low(to_f32<DT>((e & 1) ? a[e >> 1] >> 16 : a[e >> 1] & 0xffffu));
-      }
+  static __device__ __forceinline__ u32x4 raw(const S* x, int i, int n) {
+    if constexpr (!TINY) {
+      return ld16h(x + min(i, n - EPL));
     } else {
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) v[e] = i + e < n ? load1<DT>(x, i + e) : kNegInf;
+      u32x4 r = {0u, 0u, 0u, 0u};
+      for (int e = 0; e < n; ++e) put(r, e, x[e]);
+      return r;
     }
+  }
+  static __device__ __forceinline__ void put(u32x4& r, int e, S b) {
+#pragma unroll
+    for (int q = 0; q < EPL; ++q)
+      if (q == e) {
+        if constexpr (DT == kF32) r[q] = __float_as_uint(b);
+        else r[q >> 1] = (q & 1) ? (r[q >> 1] & 0xffffu) | ((uint32_t)b << 16)
+                                 : (r[q >> 1] & 0xffff0000u) | (uint32_t)b;
+      }
+  }
+  // what raw(x, i, n) loaded, its elements at their places and -inf from `end` on
+  static __device__ __forceinline__ u32x4 fix(u32x4 r, int i, int n, int end) {
+    constexpr uint32_t LOW = DT == kF32 ? 0xff800000u : DT == kF16 ? 0xfc00u : 0xff80u;
+    const int by = TINY ? 0 : i - min(i, n - EPL);  // places the load began too early
+    u32x4 o = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      uint32_t b = LOW;
+#pragma unroll
+      for (int q = 0; q < EPL; ++q) {
+        const uint32_t w = DT == kF32 ? r[q & 3] : (q & 1) ? r[q >> 1] >> 16 : r[q >> 1] & 0xffffu;
+        if (q == e + by && i + e < end) b = w;
+      }
+      if constexpr (DT == kF32) o[e & 3] = b;
+      else o[e >> 1] |= b << (16 * (e & 1));
+    }
+    return o;
+  }
+  static __device__ __forceinline__ float value(const u32x4& r, int e) {
+    if constexpr (DT == kF32) return nan_to_low(__uint_as_float(r[e]));
+    else return nan_to_low(to_f32<DT>((e & 1) ? r[e >> 1] >> 16 : r[e >> 1] & 0xffffu));
+  }
+  // `last`: the wave's last element, plus one
+  __device__ __forceinline__ void take(u32x4 r, int i, int n, int end, int last) {
+    if (TINY || last > end) r = fix(r, i, n, end);  // uniform
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) v[e] = value(r, e);
   }
 };
 
@@ -149,94 +204,99 @@ __device__ __forceinline__ T wave_sum(T v) {
   for (int s = 1; s < 64; s *= 2) v += __shfl_xor(v, s);
   return v;
 }
+// Exclusive prefix sum over the wave's lanes, and the whole sum.
+__device__ __forceinline__ double wave_scan(double v, double* total) {
+  const int lane = item_id() & 63;
+  double x = v;
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) {
+    const double y = __shfl_up(x, s);
+    if (lane >= s) x += y;
+  }
+  *total = __shfl(x, 63);
+  const double e = __shfl_up(x, 1);
+  return lane == 0 ? 0.0 : e;
+}
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) v = min(v, __shfl_xor(v, s));
+  return v;
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) v = max(v, __shfl_xor(v, s));
+  return v;
+}
 
 // ---- scan --------------------------------------------------------------------------------------
-template <int DT>
+template <int DT, bool TINY>
 __global__ __launch_bounds__(256) void sample_scan_kernel(SampleParams p) {
-  constexpr int EPL = Lane<DT>::EPL, IT = kGroup / (64 * EPL);
-  const int row = wg_id_y(), chunk = wg_id_x(), tid = item_id();
-  const int lane = tid & 63, wave = tid >> 6;
+  constexpr int EPL = Lane<DT, TINY>::EPL, IT = kGroup / (64 * EPL);
+  const int row = wg_id_y(), lane = item_id() & 63;
+  const int group = __builtin_amdgcn_readfirstlane(wg_id_x() * 4 + (item_id() >> 6));
+  if (group >= p.groups) return;
   const store_t<DT>* x = reinterpret_cast<const store_t<DT>*>(p.logits) + (int64_t)row * p.ls;
-  const int base = chunk * kChunk + wave * kGroup;
-  Lane<DT> a[IT];
+  const int base = group * kGroup + lane * EPL;
+  const int end = min((group + 1) * kGroup, p.vocab);
+  u32x4 raw[IT];
 #pragma unroll
-  for (int i = 0; i < IT; ++i) a[i].load(x, base + (i * 64 + lane) * EPL, p.vocab);
+  for (int i = 0; i < IT; ++i) raw[i] = Lane<DT, TINY>::raw(x, base + i * 64 * EPL, p.vocab);
   const RowSettings s = settings(p, row);
+  Lane<DT, TINY> a[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i)
+    a[i].take(raw[i], base + i * 64 * EPL, p.vocab, end, (group + 1) * kGroup);
   float m = kNegInf;
 #pragma unroll
   for (int i = 0; i < IT; ++i)
 #pragma unroll
     for (int e = 0; e < EPL; ++e) m = fmaxf(m, a[i].v[e]);
-  m = wave_max_all(m);
-  __shared__ float wm[4];
-  __shared__ int wf[4];
-  __shared__ double wt[4], w1[4];
-  if (lane == 0) {
-    wm[wave] = m;
-    p.gmax[((int64_t)row * p.chunks + chunk) * 4 + wave] = m;
-  }
-  int first = 0x7fffffff;
-#pragma unroll
-  for (int i = IT - 1; i >= 0; --i)
-#pragma unroll
-    for (int e = EPL - 1; e >= 0; --e)
-      if (a[i].v[e] == m) first = base + (i * 64 + lane) * EPL + e;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) first = min(first, __shfl_xor(first, d));
-  if (lane == 0) wf[wave] = first;
-  __syncthreads();
-  const float cm = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-  // the weights' sum is needed unless the kept tokens are listed anyway (top-k) or the row is
-  // greedy; the sum at temperature 1 for the log-probability
-  const bool need_t = !s.greedy && s.k == 0 && s.inv != 1.0;
+  m = fmaxf(m, dpp_mov<0xb1>(m));   // quad_perm [1,0,3,2]
+  m = fmaxf(m, dpp_mov<0x4e>(m));   // quad_perm [2,3,0,1]
+  m = fmaxf(m, dpp_mov<0x124>(m));  // row_ror:4
+  m = fmaxf(m, dpp_mov<0x128>(m));  // row_ror:8: the row's maximum in each of its 16 lanes
+  if ((lane & 15) == 0) p.smax[((int64_t)row * p.groups + group) * 4 + (lane >> 4)] = m;
+  m = quad_max(m);
+  // the weights' sum is needed unless top-k lists the kept tokens anyway (or the row is greedy)
+  const bool need_t = !s.greedy && s.k == 0;
   double st = 0.0, s1 = 0.0;
-  if (cm != kNegInf) {
-    if (need_t) {
+  if (m != kNegInf && need_t) {  // uniform
+    // the elements once more, from the caches: a loop of one load's exponentials instead of
+    // sixteen in line (the code of a launch comes cold from memory)
+#pragma unroll 1
+    for (int i = 0; i < IT; ++i) {
+      Lane<DT, TINY> b;
+      const int j = base + i * 64 * EPL;
+      b.take(Lane<DT, TINY>::raw(x, j, p.vocab), j, p.vocab, end, (group + 1) * kGroup);
 #pragma unroll
-      for (int i = 0; i < IT; ++i)
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) st += weight(a[i].v[e], cm, s.inv);
+      for (int e = 0; e < EPL; ++e) st += weight(b.v[e], m, s.inv2);
     }
-    if (!s.greedy && s.k == 0 && s.inv == 1.0) {
-#pragma unroll
-      for (int i = 0; i < IT; ++i)
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) s1 += weight(a[i].v[e], cm, 1.0);
-    } else if (p.lp) {
-      // f32 exponentials (relative error about 2^-22 each, of either sign) summed in f64: the
-      // log-probability is an f32 number
-      float q = 0.f;
-#pragma unroll
-      for (int i = 0; i < IT; ++i)
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-          const float d = a[i].v[e] >= cm ? 0.f : a[i].v[e] - cm;
-          q += fast_exp2(d * 1.44269504088896340736f);
-        }
-      s1 = (double)q;
-    }
+    st = wave_sum(st);
   }
-  st = wave_sum(st);
-  s1 = wave_sum(s1);
+  if (need_t && s.t1) {
+    s1 = st;
+  } else if (p.lp && m != kNegInf) {
+    // for the log-probability, an f32 number: f32 exponentials (off by about 2^-22 of their own
+    // value, either way), 16 of them summed in f32, those sums in f64
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float d = a[i].v[e] >= m ? 0.f : a[i].v[e] - m;
+        q += fast_exp2(d * 1.44269504088896340736f);
+      }
+    s1 = wave_sum((double)q);
+  }
   if (lane == 0) {
-    wt[wave] = st;
-    w1[wave] = s1;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    const int64_t at = (int64_t)row * p.chunks + chunk;
-    const double b = (w1[0] + w1[1]) + (w1[2] + w1[3]);
-    p.sum_1[at] = b;
-    p.sum_t[at] = need_t ? (wt[0] + wt[1]) + (wt[2] + wt[3]) : b;
-    int f = 0x7fffffff;
-#pragma unroll
-    for (int w = 3; w >= 0; --w)
-      if (wm[w] == cm) f = wf[w];
-    p.first[at] = f;
+    const int64_t at = (int64_t)row * p.groups + group;
+    p.gmax[at] = m;
+    p.sum_t[at] = st;
+    p.sum_1[at] = s1;
   }
 }
 
-// ---- pick --------------------------------------------------------------------------------------
+// ---- shared by gather and pick -----------------------------------------------------------------
 // Order-preserving integers of floats (no NaN; -0 as +0), and the order of tokens as one number:
 // larger is earlier.
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -253,16 +313,13 @@ __device__ __forceinline__ float logit_of(uint64_t r) { return of_key((uint32_t)
 __device__ __forceinline__ int index_of(uint64_t r) { return (int)(0xffffffffu - (uint32_t)r); }
 
 struct PickShared {
-  uint64_t list[kList];    // ranks in index order
+  u32x4 ring[kWaves * kAhead * 64];
+  uint64_t raw[kList];     // ranks as collected
   uint64_t sorted[kList];  // ranks, earliest first
-  uint64_t wbin[kBins];    // weights in 2^-43 steps
-  uint32_t cbin[kBins];
-  double seg[kSegs];
-  double red[16];
-  int cnt[2][4][16];
-  double d[4];
-  uint64_t r[2];
-  uint32_t q[4];
+  uint32_t bin[kBins];     // counts or weights
+  double red[kWaves];
+  uint32_t cnt[kWaves];
+  int n;
   int i[8];
 };
 
@@ -274,26 +331,20 @@ __device__ __forceinline__ double block_sum(PickShared& sh, double v) {
   __syncthreads();
   double t = 0.0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) t += sh.red[w];
+  for (int w = 0; w < kWaves; ++w) t += sh.red[w];
   return t;
 }
 // Exclusive prefix sum over the workgroup's threads, and the whole sum.
 __device__ __forceinline__ double block_scan(PickShared& sh, double v, double* total) {
-  const int lane = item_id() & 63, wave = item_id() >> 6;
-  double x = v;
-#pragma unroll
-  for (int s = 1; s < 64; s *= 2) {
-    const double y = __shfl_up(x, s);
-    if (lane >= s) x += y;
-  }
-  double e = __shfl_up(x, 1);
-  if (lane == 0) e = 0.0;
+  const int wave = item_id() >> 6;
+  double mine;
+  const double e = wave_scan(v, &mine);
   __syncthreads();
-  if (lane == 63) sh.red[wave] = x;
+  if ((item_id() & 63) == 0) sh.red[wave] = mine;
   __syncthreads();
   double before = 0.0, t = 0.0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     if (w == wave) before = t;
     t += sh.red[w];
   }
@@ -305,446 +356,693 @@ __device__ __forceinline__ uint32_t block_reduce_u32(PickShared& sh, uint32_t v,
 #pragma unroll
   for (int s = 1; s < 64; s *= 2) v = f(v, (uint32_t)__shfl_xor((int)v, s));
   __syncthreads();
-  if ((item_id() & 63) == 0) sh.cnt[0][0][item_id() >> 6] = (int)v;
+  if ((item_id() & 63) == 0) sh.cnt[item_id() >> 6] = v;
   __syncthreads();
-  uint32_t t = (uint32_t)sh.cnt[0][0][0];
+  uint32_t t = sh.cnt[0];
 #pragma unroll
-  for (int w = 1; w < 16; ++w) t = f(t, (uint32_t)sh.cnt[0][0][w]);
+  for (int w = 1; w < kWaves; ++w) t = f(t, sh.cnt[w]);
   return t;
 }
 
-// Descending bitonic sort of sorted[0 .. n) padded with zeros (below every rank) to a power of two.
-__device__ __forceinline__ void sort_list(PickShared& sh, int n) {
+// Descending bitonic sort of v[0 .. n), padded with zeros to a power of two (at most kList).
+__device__ __forceinline__ void sort_list(uint64_t* v, int n) {
   int n2 = 2;
   while (n2 < n) n2 *= 2;
   const int tid = item_id();
-  for (int i = n + tid; i < n2; i += kPick) sh.sorted[i] = 0;
+  for (int i = n + tid; i < n2; i += kPick) v[i] = 0;
   __syncthreads();
-  auto step = [&](int size, int stride, int t) {
-    const int lo = 2 * t - (t & (stride - 1)), hi = lo + stride;
-    const uint64_t a = sh.sorted[lo], b = sh.sorted[hi];
-    const bool down = (lo & size) == 0;
-    if ((a < b) == down) {
-      sh.sorted[lo] = b;
-      sh.sorted[hi] = a;
-    }
-  };
-  if (n2 <= 128) {  // one wave, whose LDS accesses are in order
-    if (tid < 64)
-      for (int size = 2; size <= n2; size *= 2)
-        for (int stride = size / 2; stride > 0; stride /= 2) {
-          if (tid < n2 / 2) step(size, stride, tid);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+  for (int size = 2; size <= n2; size *= 2)
+#pragma unroll 1
+    for (int stride = size / 2; stride > 0; stride /= 2) {
+#pragma unroll 1
+      for (int t = tid; t < n2 / 2; t += kPick) {
+        const int lo = 2 * t - (t & (stride - 1)), hi = lo + stride;
+        const uint64_t a = v[lo], b = v[hi];
+        if ((a < b) == ((lo & size) == 0)) {
+          v[lo] = b;
+          v[hi] = a;
         }
-    __syncthreads();
-  } else {
-    for (int size = 2; size <= n2; size *= 2)
-      for (int stride = size / 2; stride > 0; stride /= 2) {
-        for (int t = tid; t < n2 / 2; t += kPick) step(size, stride, t);
-        __syncthreads();
       }
-  }
+      __syncthreads();
+    }
 }
 
-template <int DT>
+// A row, or a part of one: each wave owns a run of whole steps (64 lanes' loads).
+template <int DT, bool TINY>
 struct Row {
-  static constexpr int EPL = Lane<DT>::EPL;
-  static constexpr int TILE = kPick * EPL;
+  static constexpr int EPL = Lane<DT, TINY>::EPL;
+  static constexpr int STEP = 64 * EPL;
   const store_t<DT>* x;
   int n;
-  // f(index, logit) of every element, in no order
+  u32x4* ring;  // LDS
+  // the run of wave w when [from, to) is shared out: steps of it, the last waves' may be empty
+  static __device__ __forceinline__ int run_of(int from, int to) {
+    const int steps = (to - from + STEP - 1) / STEP;
+    return (steps + kWaves - 1) / kWaves * STEP;
+  }
+  // f(this lane's first index, its EPL logits) over the wave's run of [from, to) in index order, a
+  // step at a time, elements past `to` as -inf. kAhead steps are loaded while as many are worked on:
+  // a CU alone reads a row (200 KB or so) from beyond its L2. The ones worked on lie in the wave's
+  // part of `ring`, so that f is there once, in a loop over them (in registers every step would have
+  // its own copy of f; turning registers round instead waits for the load just issued).
+  template <class F>
+  __device__ __forceinline__ void each(int from, int to, F f) const {
+    const int run = run_of(from, to);
+    const int wave = __builtin_amdgcn_readfirstlane(item_id() >> 6), lane = item_id() & 63;
+    const int a = from + wave * run, b = min(to, a + run);
+    const int off = lane * EPL;
+    u32x4* mine = ring + wave * (kAhead * 64) + lane;
+    u32x4 r[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) r[j] = Lane<DT, TINY>::raw(x, a + j * STEP + off, n);
+#pragma unroll 1
+    for (int i = a; i < b; i += kAhead * STEP) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) mine[j * 64] = r[j];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        r[j] = Lane<DT, TINY>::raw(x, i + (kAhead + j) * STEP + off, n);
+#pragma unroll 1
+      for (int j = 0; j < kAhead && i + j * STEP < b; ++j) {  // uniform
+        Lane<DT, TINY> cur;
+        cur.take(mine[j * 64], i + j * STEP + off, n, b, i + (j + 1) * STEP);
+        f(i + j * STEP + off, cur);
+      }
+    }
+  }
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    constexpr int U = 4;  // tiles whose loads are in flight together
-#pragma unroll 1
-    for (int b = item_id() * EPL; b < n; b += U * TILE) {
-      Lane<DT> a[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) a[j].load(x, min(b + j * TILE, n), n);
-#pragma unroll
-      for (int j = 0; j < U; ++j)
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) f(b + j * TILE + e, a[j].v[e]);
-    }
+    each(0, n, f);
   }
 };
 
-// The ranks of the elements that `take` chooses, in index order, to sh.list (the first kList of
-// them) and sh.sorted alike. Returns how many there are. One barrier per U tiles: each wave says
-// how many it keeps of each tile, and every thread adds up what lies before its own.
-template <int DT, class F>
-__device__ __forceinline__ int collect(const Row<DT>& row, PickShared& sh, F take) {
-  constexpr int EPL = Row<DT>::EPL, TILE = Row<DT>::TILE, U = 4;
-  const int tid = item_id(), lane = tid & 63, wave = tid >> 6;
-  const uint64_t below = (uint64_t(1) << lane) - 1;
-  int n = 0, flip = 0;
-  __syncthreads();
-#pragma unroll 1
-  for (int b0 = 0; b0 < row.n; b0 += U * TILE) {
-    Lane<DT> a[U];
-#pragma unroll
-    for (int j = 0; j < U; ++j) a[j].load(row.x, min(b0 + j * TILE + tid * EPL, row.n), row.n);
-    uint32_t mine = 0;  // bit j * EPL + e
-    int before[U];
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      int all = 0;
-      before[j] = 0;
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) {
-        const float l = a[j].v[e];
-        const bool t = l != kNegInf && take(b0 + j * TILE + tid * EPL + e, l);
-        const uint64_t v = __ballot(t);
-        before[j] += __popcll(v & below);
-        all += __popcll(v);
-        mine |= (uint32_t)t << (j * EPL + e);
-      }
-      if (lane == 0) sh.cnt[flip][j][wave] = all;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      int at = n + before[j];
-#pragma unroll
-      for (int w = 0; w < 16; ++w) {
-        const int c = sh.cnt[flip][j][w];
-        if (w < wave) at += c;
-        n += c;
-      }
-      if ((mine >> (j * EPL)) & ((1u << EPL) - 1)) {
-#pragma unroll
-        for (int e = 0; e < EPL; ++e)
-          if ((mine >> (j * EPL + e)) & 1) {
-            if (at < kList) {
-              const uint64_t r = rank_of(a[j].v[e], b0 + j * TILE + tid * EPL + e);
-              sh.list[at] = r;
-              sh.sorted[at] = r;
-            }
-            ++at;
-          }
-      }
-    }
-    flip ^= 1;
-  }
-  __syncthreads();
-  return n;
+// Appends the lanes' ranks where `take`, in no order; sh.n counts them, the first kList are held.
+__device__ __forceinline__ void append(PickShared& sh, bool take, float l, int i) {
+  const uint64_t v = __ballot(take);
+  if (v == 0) return;  // uniform
+  const int lane = item_id() & 63;
+  int at = 0;
+  if (lane == 0) at = atomicAdd(&sh.n, __popcll(v));
+  at = __builtin_amdgcn_readfirstlane(at) + __popcll(v & ((uint64_t(1) << lane) - 1));
+  if (take && at < kList) sh.raw[at] = rank_of(l, i);
 }
 
-// The element at which the running weight passes u times the whole, over elements in order: `w`
-// (0 for one that is not kept) of PER consecutive positions per thread. Every thread returns the
-// position (threads' elements are PER * tid + e).
+// One wave: the position at which the running weight passes u times the whole, over positions
+// PER * lane + e in order; the last one of any weight where rounding leaves none.
 template <int PER>
-__device__ __forceinline__ int draw(PickShared& sh, const double (&w)[PER], double u) {
+__device__ __forceinline__ int wave_draw(const double (&w)[PER], double u) {
   double mine = 0.0, total;
 #pragma unroll
   for (int e = 0; e < PER; ++e) mine += w[e];
-  double run = block_scan(sh, mine, &total);
+  double run = wave_scan(mine, &total);
   const double target = u * total;
-  if (item_id() == 0) {
-    sh.i[6] = 0x7fffffff;
-    sh.i[7] = -1;
-  }
-  __syncthreads();
+  const int lane = item_id() & 63;
+  int hit = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int e = PER - 1; e >= 0; --e)
+    if (last < 0 && w[e] > 0.0) last = PER * lane + e;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     run += w[e];
-    if (w[e] > 0.0) {
-      if (run > target) atomicMin(&sh.i[6], PER * (int)item_id() + e);
-      atomicMax(&sh.i[7], PER * (int)item_id() + e);
-    }
+    if (w[e] > 0.0 && run > target) hit = min(hit, PER * lane + e);
   }
-  __syncthreads();
-  // (rounding may leave every running sum at or below u times the whole: then the last one)
-  const int at = sh.i[6];
-  const int last = sh.i[7];
-  __syncthreads();
-  return at != 0x7fffffff ? at : last;
+  hit = wave_min(hit);
+  last = wave_max(last);
+  return hit != 0x7fffffff ? hit : last;
 }
 
-// What is kept of a row: ranks from `low` up, of weight at least mp.
-struct Kept {
-  uint64_t low;
-  double mp;
-};
-
-// The token of a row whose every kept element is in sh.list[0 .. n): the definition as it stands.
-// whole: W(S1) where S1 reaches below the list (top_k and min_p off), else negative.
-__device__ int pick_from_list(PickShared& sh, int n, const RowSettings& s, float m, double whole,
-                              double u) {
-  sort_list(sh, n);
+// The token of a row all of whose kept elements are among sh.raw[0 .. n), n <= kShort: the
+// definition as it stands. whole: W(S1) where S1 reaches below the list, else negative. The
+// result is wave 0's alone.
+__device__ __forceinline__ int pick_short(PickShared& sh, int n, const RowSettings& s, float m,
+                                          double whole, double u) {
+  // both orders by counting: kPick / n2 threads an element (n2: n as a power of two), each a part of
+  // the list; an element's place is the number of ranks above (indexes below) its own
   const int tid = item_id();
-  double w[2];
-  bool in1[2];
+  int n2 = 64;
+  while (n2 < n) n2 *= 2;
+  const int parts = kPick / n2, part = tid / n2, me = tid % n2;  // parts 16, 8 or 4
+  uint32_t* place = sh.bin;  // [part][me]: by rank (low half) and by index (high half)
+  {
+    const uint64_t mine = me < n ? sh.raw[me] : 0;
+    const uint32_t my_i = (uint32_t)mine;
+    const int len = n2 / parts, a = part * len, b = min(a + len, n);
+    uint32_t c = 0;
+#pragma unroll 4
+    for (int j = a; j < b; ++j) {
+      const uint64_t r = sh.raw[j];
+      c += (r > mine ? 1u : 0u) + ((uint32_t)r > my_i ? 0x10000u : 0u);  // (indexes are inverted)
+    }
+    place[part * n2 + me] = c;
+    __syncthreads();
+    if (part == 0 && me < n) {
+      c = 0;
+      for (int q = 0; q < parts; ++q) c += place[q * n2 + me];
+      sh.sorted[c & 0xffffu] = mine;
+      sh.sorted[kShort + (c >> 16)] = mine;  // in index order
+    }
+    __syncthreads();
+  }
+  if (tid >= 64) return 0;
+  constexpr int PER = kShort / 64;
+  double w[PER];
+  double sum = 0.0, total;
+  bool in1[PER];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int j = 2 * tid + e;
-    w[e] = j < n ? weight(logit_of(sh.sorted[j]), m, s.inv) : 0.0;
+  for (int e = 0; e < PER; ++e) {
+    const int j = PER * tid + e;
+    w[e] = j < n ? weight(logit_of(sh.sorted[j]), m, s.inv2) : 0.0;
     in1[e] = j < n && (s.k == 0 || j < s.k) && w[e] >= s.mp;
     if (!in1[e]) w[e] = 0.0;
+    sum += w[e];
   }
-  double total;
-  const double before = block_scan(sh, w[0] + w[1], &total);
+  double run = wave_scan(sum, &total);
   const double limit = (double)s.p * (whole >= 0.0 ? whole : total);
-  // the last rank that is kept (in1 and the running weight make it a run from the first)
-  if (tid == 0) sh.i[5] = 0;
-  __syncthreads();
+  // the kept ranks are a run from the first: its last one
+  int last = 0;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const double b = e == 0 ? before : before + w[0];
-    if (in1[e] && (s.p >= 1.f || b < limit)) atomicMax(&sh.i[5], 2 * tid + e);
+  for (int e = 0; e < PER; ++e) {
+    if (in1[e] && (s.p >= 1.f || run < limit)) last = PER * tid + e;
+    run += w[e];
   }
-  __syncthreads();
-  const uint64_t low = sh.sorted[sh.i[5]];
+  const uint64_t low = sh.sorted[wave_max(last)];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int j = 2 * tid + e;
-    const uint64_t r = j < n ? sh.list[j] : 0;
-    w[e] = r >= low && j < n ? weight(logit_of(r), m, s.inv) : 0.0;
+  for (int e = 0; e < PER; ++e) {
+    const int j = PER * tid + e;
+    const uint64_t r = j < n ? sh.sorted[kShort + j] : 0;
+    w[e] = j < n && r >= low ? weight(logit_of(r), m, s.inv2) : 0.0;
   }
-  return index_of(sh.list[draw<2>(sh, w, u)]);
+  return index_of(sh.sorted[kShort + wave_draw<PER>(w, u)]);
 }
 
-// The last rank that is kept when ranks `from` and earlier of weight >= mp are cut at a count
-// (by_count: the first `count`) or at a weight (those whose predecessors weigh less than `limit`).
-// Histograms over the logits, first linear below m, then over ever smaller ranges of their integer
-// keys, until the boundary's bin holds a list's worth of tokens or a single value.
-template <int DT>
-__device__ uint64_t boundary(const Row<DT>& row, PickShared& sh, float m, double inv, Kept from,
-                             bool by_count, int count, double limit) {
+// The last rank that is kept when a row's ranks are cut at a count (by_count: the first `count`) or
+// at a weight (those whose predecessors weigh less than `limit`). Histograms over the logits, first
+// linear below m, then over ever smaller ranges of their integer keys, until the boundary's bin
+// holds a list's worth of tokens or a single value. total_w: the row's weight.
+// *listed (weights only): the boundary's bin is listed, sh.sorted[0 .. *listed), and `mine` is the
+// weight of the ranks before that bin in the wave's run of the row; -1 where it is not.
+template <int DT, bool TINY>
+__device__ __forceinline__ uint64_t boundary(const Row<DT, TINY>& row, PickShared& sh, float m,
+                                             double inv2, bool by_count, int count, double limit,
+                                             double total_w, int* listed, double* mine_before) {
+  constexpr int EPL = Row<DT, TINY>::EPL;
   const int tid = item_id();
-  // linear bins: 1/64 of a natural-log unit of weight, or of a logit
-  const float scale = by_count ? 64.f : fminf(64.f * (float)inv, 1e30f);
+  // linear bins: 1/256 of a natural-log unit of weight, or 1/128 of a logit
+  const float scale = by_count ? 128.f : fminf((float)(inv2 * (256.0 / kLog2e)), 1e30f);
+  const float inv2f = fminf((float)inv2, 1e30f);
+  // histogram weights are integers whose sum over the row stays below 2^31
+  const int wshift = 30 - (int)__builtin_ceil(log2(fmax(total_w, 1.0)));
+  const float wscale = __builtin_ldexpf(1.f, wshift);
   uint32_t klo = key_of(kNegInf) + 1, khi = key_of(m);  // the range that holds the boundary
   int shift = -1;                                       // -1: linear bins
-  // a bin index grows towards earlier ranks for integer bins, towards later ones for linear bins;
-  // `bin` below is turned so that 0 is always the earliest
-  auto member = [&](int i, float l) {
-    if (rank_of(l, i) < from.low) return false;
-    return from.mp <= 0.0 || weight(l, m, inv) >= from.mp;
-  };
+  *listed = -1;
 #pragma unroll 1
   for (;;) {
-    auto bin_of = [&](float l) -> int {
-      if (shift < 0) {
-        const float d = (m - l) * scale;  // NaN only for two infinities: l = m then
-        return l >= m ? 0 : d >= (float)(kBins - 1) ? kBins - 1 : (int)d;
+    // bin 0 is the earliest; bins grow as logits fall
+    auto linear_bin = [&](float l) -> int {
+      return (int)(l >= m ? 0.f : fminf((m - l) * scale, (float)(kBins - 1)));
+    };
+    // the least key of bins [0, b]
+    auto bin_floor = [&](int b) -> uint32_t {
+      if (shift >= 0) {
+        const uint64_t d = ((uint64_t)(b + 1) << shift) - 1;
+        return d >= khi - klo ? klo : khi - (uint32_t)d;
       }
-      return (int)((khi - key_of(l)) >> shift);
+      uint32_t x = klo, y = khi;  // by bisection: the bin is monotone in the logit
+      while (x < y) {
+        const uint32_t mid = x + (y - x) / 2;
+        if (linear_bin(of_key(mid)) <= b) y = mid;
+        else x = mid + 1;
+      }
+      return x;
     };
-    auto inside = [&](float l) {
-      const uint32_t k = key_of(l);
-      return k >= klo && k <= khi;
-    };
+    const bool counts = by_count || shift == 0;  // (a single value's weight is count * weight)
+    const float fhi = of_key(khi), flo = of_key(klo);
     __syncthreads();
-    for (int b = tid; b < kBins; b += kPick) {
-      sh.wbin[b] = 0;
-      sh.cbin[b] = 0;
-    }
+    for (int b = tid; b < kBins; b += kPick) sh.bin[b] = 0;
     __syncthreads();
-    double above = 0.0;     // weight of the earlier ranks, past the range
-    uint32_t n_above = 0;   // and their number
-    row.each([&](int i, float l) {
-      if (l == kNegInf || !member(i, l)) return;
-      if (key_of(l) > khi) {
-        ++n_above;
-        if (!by_count) above += weight(l, m, inv);
-      } else if (inside(l)) {
-        const int b = bin_of(l);
-        atomicAdd(&sh.cbin[b], 1u);
-        if (!by_count)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.wbin[b]),
-                    (unsigned long long)(weight(l, m, inv) * 0x1p43));
+    double above = 0.0;    // weight of the ranks before the range (integer bins only)
+    uint32_t n_above = 0;  // and their number
+    row.each([&](int, const Lane<DT, TINY>& a) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float l = a.v[e];
+        if (shift >= 0) {  // uniform
+          n_above += l > fhi ? 1u : 0u;
+          if (!by_count && __ballot(l > fhi)) above += l > fhi ? weight(l, m, inv2) : 0.0;
+        }
+        // an f32 exponential, off by up to (|y| + 2) 2^-23: 2^-18 of it where it counts
+        const float w = l >= m ? wscale : fast_exp2((l - m) * inv2f) * wscale;
+        const int b = shift < 0 ? linear_bin(l) : (int)((khi - key_of(l)) >> (shift & 31));
+        if (l >= flo && l <= fhi) atomicAdd(&sh.bin[b], counts ? 1u : (uint32_t)w);
       }
     });
-    if (!by_count) above = block_sum(sh, above);
-    n_above = block_reduce_u32(sh, n_above, [](uint32_t a, uint32_t b) { return a + b; });
-    // ---- walk the bins from the earliest (thread t: bins 2 t, 2 t + 1): by weight the boundary is
-    // in bins [lo, hi], where the running weight passes the limit less and more the integers'
-    // possible error (2^-43 an element) and the sums' own; at single-value bins the weights are
-    // count * weight, exact
-    double w[2];
+    if (!by_count && shift >= 0) above = block_sum(sh, above);
+    if (shift >= 0)
+      n_above = block_reduce_u32(sh, n_above, [](uint32_t a, uint32_t b) { return a + b; });
+    else __syncthreads();
+    // ---- walk the bins from the earliest (thread t: bins PB t ..): by weight the boundary is in
+    // bins [lo, hi], where the running weight passes the limit less and more what the histogram's
+    // weights may be off by; at single-value bins the weights are exact
+    constexpr int PB = kBins / kPick;
+    double w[PB];
+    double sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int b = 2 * tid + e;
-      const uint32_t c = sh.cbin[b];
-      w[e] = by_count     ? (double)c
-             : shift == 0 ? (double)c * weight(of_key(khi - (uint32_t)min((uint32_t)b, khi - klo)), m, inv)
-                          : (double)sh.wbin[b] * 0x1p-43;
+    for (int e = 0; e < PB; ++e) {
+      const int b = PB * tid + e;
+      const double c = (double)sh.bin[b];
+      w[e] = by_count     ? c
+             : shift == 0 ? c * weight(of_key(khi - min((uint32_t)b, khi - klo)), m, inv2)
+                          : __builtin_ldexp(c, -wshift);
+      sum += w[e];
     }
     double total;
-    double run = block_scan(sh, w[0] + w[1], &total);
+    double run = block_scan(sh, sum, &total);
     run += by_count ? (double)n_above : above;
     const double want = by_count ? (double)count : limit;
-    const double slack = by_count || shift == 0 ? 0.0 : (above + total + 1.0) * 1e-12 + row.n * 0x1p-42;
+    // (an integer weight is truncated: one step an element)
+    const double slack = counts ? 0.0 : (above + total) * 0x1p-17 + __builtin_ldexp(row.n, -wshift);
     if (tid == 0) {
       sh.i[0] = kBins;  // lo
       sh.i[1] = kBins;  // hi
-      sh.i[2] = 0;      // the last bin with a member
+      sh.i[2] = 0;      // the last bin with a weight
+      sh.n = 0;
     }
     __syncthreads();
+    {
+      int b0 = kBins, b1 = kBins, b2 = 0;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int b = 2 * tid + e;
-      run += w[e];
-      if (sh.cbin[b]) {
-        if (run >= want - slack) atomicMin(&sh.i[0], b);
-        if (run >= want + slack) atomicMin(&sh.i[1], b);
-        atomicMax(&sh.i[2], b);
+      for (int e = 0; e < PB; ++e) {
+        const int b = PB * tid + e;
+        run += w[e];
+        if (run >= want - slack) b0 = min(b0, b);
+        if (run >= want + slack) b1 = min(b1, b);
+        if (sh.bin[b]) b2 = b;
+      }
+      // (within a wave first: a thousand atomics on one word took 17 us)
+      b0 = wave_min(b0);
+      b1 = wave_min(b1);
+      b2 = wave_max(b2);
+      if ((tid & 63) == 0) {
+        atomicMin(&sh.i[0], b0);
+        atomicMin(&sh.i[1], b1);
+        atomicMax(&sh.i[2], b2);
       }
     }
     __syncthreads();
-    const int last = sh.i[2];
-    const int hi = min(sh.i[1], last), lo = min(sh.i[0], hi);
-    uint32_t pop = 0, pre = 0;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int b = 2 * tid + e;
-      if (b >= lo && b <= hi) pop += sh.cbin[b];
-      if (b < lo) pre += sh.cbin[b];
-    }
-    pop = block_reduce_u32(sh, pop, [](uint32_t a, uint32_t b) { return a + b; });
-    pre = block_reduce_u32(sh, pre, [](uint32_t a, uint32_t b) { return a + b; });
+    // (a count that the row does not reach ends at its last element; a limit that it does not
+    // reach but for rounding, somewhere from the last bin of any weight on)
+    int hi = sh.i[1] == kBins ? (counts ? sh.i[2] : kBins - 1) : sh.i[1];
+    int lo = min(sh.i[0] == kBins ? sh.i[2] : sh.i[0], hi);
 
-    if (pop <= (uint32_t)kList) {
-      // ---- the boundary is one of these: sorted, and the definition applied to them
-      double ab = 0.0;
-      if (!by_count) {
-        row.each([&](int i, float l) {
-          if (l == kNegInf || !member(i, l)) return;
-          if (key_of(l) > khi || (inside(l) && bin_of(l) < lo)) ab += weight(l, m, inv);
-        });
-        ab = block_sum(sh, ab);
-      }
-      const int n = collect(row, sh, [&](int i, float l) {
-        if (!inside(l) || !member(i, l)) return false;
-        const int b = bin_of(l);
-        return b >= lo && b <= hi;
-      });
-      sort_list(sh, n);
-      double wl[2];
+    // ---- what the bins hold is listed; the same pass sums what comes before
+    uint32_t top = lo == 0 ? khi : bin_floor(lo - 1) - 1, bottom = bin_floor(hi);
+    {
+      const float ftop = of_key(top), fbottom = of_key(bottom);
+      double x = 0.0;
+      uint32_t pre = 0;
+      row.each([&](int i, const Lane<DT, TINY>& a) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = 2 * tid + e;
-        wl[e] = j >= n ? 0.0 : by_count ? 1.0 : weight(logit_of(sh.sorted[j]), m, inv);
+        for (int e = 0; e < EPL; ++e) {
+          const float l = a.v[e];
+          append(sh, l >= fbottom && l <= ftop, l, i + e);
+          if (by_count) pre += l > ftop ? 1u : 0u;
+          else if (__ballot(l > ftop)) x += l > ftop ? weight(l, m, inv2) : 0.0;
+        }
+      });
+      if (by_count)
+        pre = block_reduce_u32(sh, pre, [](uint32_t a, uint32_t b) { return a + b; });
+      x = wave_sum(x);
+      *mine_before = x;
+      above = by_count ? (double)pre : block_sum(sh, (tid & 63) == 0 ? x : 0.0);
+    }
+    const int n = sh.n;
+    if (n <= kList) {
+      // ---- the boundary is one of these: ordered, and the definition applied to them
+      __syncthreads();
+      for (int j = tid; j < n; j += kPick) sh.sorted[j] = sh.raw[j];
+      __syncthreads();
+      sort_list(sh.sorted, n);
+      if (!by_count) *listed = n;
+      constexpr int PL = kList / kPick;
+      double wl[PL];
+      double mine = 0.0, tot;
+#pragma unroll
+      for (int e = 0; e < PL; ++e) {
+        const int j = PL * tid + e;
+        wl[e] = j >= n ? 0.0 : by_count ? 1.0 : weight(logit_of(sh.sorted[j]), m, inv2);
+        mine += wl[e];
       }
-      double tot;
-      const double before = block_scan(sh, wl[0] + wl[1], &tot) +
-                            (by_count ? (double)(n_above + pre) : ab);
+      double before = above + block_scan(sh, mine, &tot);
       if (tid == 0) sh.i[3] = 0;
       __syncthreads();
+      int at = 0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const double b = e == 0 ? before : before + wl[0];
-        if (2 * tid + e < n && b < want) atomicMax(&sh.i[3], 2 * tid + e);
+      for (int e = 0; e < PL; ++e) {
+        if (PL * tid + e < n && before < want) at = PL * tid + e;
+        before += wl[e];
       }
+      at = wave_max(at);
+      if ((tid & 63) == 0) atomicMax(&sh.i[3], at);
       __syncthreads();
       const uint64_t r = sh.sorted[sh.i[3]];
       __syncthreads();
       return r;
     }
-    if (shift == 0 && lo == hi) {
+    if (top == bottom) {
       // ---- one value, more often than a list holds: its t-th occurrence in index order
-      const uint32_t key = khi - (uint32_t)lo;
-      const float v = of_key(key);
-      const double wv = by_count ? 1.0 : weight(v, m, inv);
-      double ab = (double)n_above + (double)pre;
-      if (!by_count) {
-        // above + the earlier bins, in the walk's arithmetic
-        double x = 0.0;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (2 * tid + e < lo) x += w[e];
-        ab = above + block_sum(sh, x);
-      }
-      // kept: occurrences j with ab + j wv < want
-      double t = ab < want ? (double)pop : 1.0;
+      const float v = of_key(top);
+      const double wv = by_count ? 1.0 : weight(v, m, inv2);
+      // kept: occurrences j with above + j wv < want
+      double t = above < want ? (double)n : 1.0;
       if (wv > 0.0) {
-        t = fmin(fmax(__builtin_ceil((want - ab) / wv), 1.0), (double)pop);
-        if (t > 1.0 && ab + (t - 1.0) * wv >= want) t -= 1.0;
-        else if (ab + t * wv < want) t += 1.0;
+        t = fmin(fmax(__builtin_ceil((want - above) / wv), 1.0), (double)n);
+        if (t > 1.0 && above + (t - 1.0) * wv >= want) t -= 1.0;
+        else if (above + t * wv < want) t += 1.0;
       }
-      const uint32_t nth = (uint32_t)fmin(fmax(t, 1.0), (double)pop);
-      // its index: counted tile by tile
-      constexpr int EPL = Row<DT>::EPL, TILE = Row<DT>::TILE;
-      const int lane = tid & 63, wave = tid >> 6;
-      uint32_t seen = 0;
+      const uint32_t nth = (uint32_t)fmin(fmax(t, 1.0), (double)n);
+      // its index: the waves' counts, then the wave that holds it step by step
+      uint32_t mine = 0;
+      row.each([&](int, const Lane<DT, TINY>& a) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) mine += a.v[e] == v ? 1u : 0u;
+      });
+      double all, wave_all;
+      const double wave_mine = wave_sum((double)mine);
+      const double first = block_scan(sh, (tid & 63) == 0 ? wave_mine : 0.0, &all);
+      // (the scan gives lane 0 of a wave the waves before it)
+      uint32_t seen = (uint32_t)__shfl(first, 0);
       if (tid == 0) sh.i[4] = 0;
-#pragma unroll 1
-      for (int b = 0; b < row.n; b += TILE) {
-        Lane<DT> a;
-        const int i0 = b + tid * EPL;
-        a.load(row.x, min(i0, row.n), row.n);
-        uint32_t mine = 0;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e)
-          mine += i0 + e < row.n && a.v[e] != kNegInf && key_of(a.v[e]) == key && member(i0 + e, a.v[e]);
-        uint32_t inc = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const uint32_t y = (uint32_t)__shfl_up((int)inc, d);
-          if (lane >= d) inc += y;
-        }
-        __syncthreads();
-        if (lane == 63) sh.cnt[0][0][wave] = (int)inc;
-        __syncthreads();
-        uint32_t before = seen + inc - mine, all = 0;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          if (x < wave) before += (uint32_t)sh.cnt[0][0][x];
-          all += (uint32_t)sh.cnt[0][0][x];
-        }
-#pragma unroll
-        for (int e = 0; e < EPL; ++e)
-          if (i0 + e < row.n && a.v[e] != kNegInf && key_of(a.v[e]) == key && member(i0 + e, a.v[e]))
-            if (++before == nth) sh.i[4] = i0 + e;
-        seen += all;
-        if (seen >= nth) break;  // uniform
-      }
       __syncthreads();
-      const uint64_t r = ((uint64_t)key << 32) | (0xffffffffu - (uint32_t)sh.i[4]);
+      if (seen < nth && nth <= seen + (uint32_t)wave_mine)
+        row.each([&](int i, const Lane<DT, TINY>& a) {
+          uint32_t c = 0;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) c += a.v[e] == v ? 1u : 0u;
+          uint32_t before = seen + (uint32_t)wave_scan((double)c, &wave_all);
+#pragma unroll
+          for (int e = 0; e < EPL; ++e)
+            if (a.v[e] == v)
+              if (++before == nth) sh.i[4] = i + e;
+          seen += (uint32_t)wave_all;
+        });
+      __syncthreads();
+      const uint64_t r = ((uint64_t)top << 32) | (0xffffffffu - (uint32_t)sh.i[4]);
       __syncthreads();
       return r;
     }
-    // ---- a smaller range: the keys of bins [lo, hi]
-    uint32_t a = 0xffffffffu, b = 0;
-    row.each([&](int i, float l) {
-      if (l == kNegInf || !inside(l) || !member(i, l)) return;
-      const int bb = bin_of(l);
-      if (bb >= lo && bb <= hi) {
-        a = min(a, key_of(l));
-        b = max(b, key_of(l));
-      }
-    });
-    a = block_reduce_u32(sh, a, [](uint32_t x, uint32_t y) { return min(x, y); });
-    b = block_reduce_u32(sh, b, [](uint32_t x, uint32_t y) { return max(x, y); });
-    klo = a;
-    khi = b;
+    // ---- a smaller range. First the one bin of [lo, hi], by exact sums (so that every round leaves
+    // a bin of the last one's, and the rounds end)
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      const float fm = of_key(bin_floor(mid));
+      double y = 0.0;
+      row.each([&](int, const Lane<DT, TINY>& a) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+          if (__ballot(a.v[e] >= fm)) y += a.v[e] >= fm ? weight(a.v[e], m, inv2) : 0.0;
+      });
+      if (block_sum(sh, y) >= want) hi = mid;
+      else lo = mid + 1;
+    }
+    top = lo == 0 ? khi : bin_floor(lo - 1) - 1;
+    klo = bin_floor(lo);
+    khi = top;
     const int bits = 32 - __builtin_clz((khi - klo) | 1u);
-    shift = max(0, bits - 11);
+    shift = max(0, bits - 12);
   }
 }
 
-template <int DT>
+// Any filters, any number of kept tokens. The result is every thread's.
+template <int DT, bool TINY>
+__device__ __forceinline__ int pick_wide(const Row<DT, TINY>& row, PickShared& sh, const RowSettings& s,
+                                         float m, double W, double u) {
+  constexpr int EPL = Row<DT, TINY>::EPL;
+  const int tid = item_id(), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint64_t low = 0;  // kept: ranks from here up, of weight >= mp
+  int listed = -1;
+  double mine = 0.0;
+  auto kept_weight = [&](int i, float l) {
+    const bool in = rank_of(l, i) >= low;
+    if (!__ballot(in)) return 0.0;
+    const double w = in ? weight(l, m, s.inv2) : 0.0;
+    return w >= s.mp ? w : 0.0;
+  };
+  // the cut by count, then the one by weight (one loop, so that the code is there once)
+#pragma unroll 1
+  for (int by = s.k > 0 ? 0 : 1; by < (s.p < 1.f ? 2 : 1); ++by) {
+    double limit = 0.0, all = 1.0;
+    if (by == 1) {
+      // W(S1) and the whole row's weight
+      double w1 = all = W;
+      if (s.k > 0 || s.mp > 0.0) {
+        double x = 0.0, y = 0.0;
+        row.each([&](int i, const Lane<DT, TINY>& a) {
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) {
+            const double w = weight(a.v[e], m, s.inv2);
+            y += w;
+            if (w >= s.mp && rank_of(a.v[e], i + e) >= low) x += w;
+          }
+        });
+        w1 = block_sum(sh, x);
+        all = block_sum(sh, y);
+      }
+      limit = (double)s.p * w1;
+    }
+    // S1 is a run from the first rank and weighs more than the limit (p < 1), so the boundary in
+    // the whole row's order is the boundary in S1's; a limit of 0 or less keeps the first alone
+    const uint64_t r = boundary(row, sh, m, s.inv2, by == 0, s.k, limit, all, &listed, &mine);
+    if (r > low) low = r;
+    else listed = -1;
+  }
+  // ---- the kept weight of each wave's run; then of the runs of the run that holds u times the
+  // whole, down to 256 elements
+  int from = 0, to = row.n;
+  bool known = false;
+  if (listed >= 0 && s.mp <= 0.0) {
+    // what comes before the boundary's bin is known; its kept ranks join their runs
+    const int run = Row<DT, TINY>::run_of(0, row.n);
+    double x = 0.0;
+#pragma unroll 1
+    for (int j = lane; j < listed; j += 64) {
+      const uint64_t r = sh.sorted[j];
+      if (r >= low && index_of(r) / run == wave) x += weight(logit_of(r), m, s.inv2);
+    }
+    mine += wave_sum(x);
+    known = true;
+  }
+  double left = 0.0;
+  bool top = true;
+#pragma unroll 1
+  for (;;) {
+    if (!known) {
+      double x = 0.0;
+      row.each(from, to, [&](int i, const Lane<DT, TINY>& a) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x += kept_weight(i + e, a.v[e]);
+      });
+      mine = wave_sum(x);
+    }
+    known = false;
+    __syncthreads();
+    if (lane == 0) sh.red[wave] = mine;
+    __syncthreads();
+    double total = 0.0;
+#pragma unroll 1
+    for (int w = 0; w < kWaves; ++w) total += sh.red[w];
+    if (top) left = u * total;
+    top = false;
+    // the first run whose running weight passes `left`, the last one of any weight where rounding
+    // leaves none
+    double run = 0.0, before = 0.0;
+    int hit = 0;
+    bool found = false;
+#pragma unroll 1
+    for (int w = 0; w < kWaves; ++w) {
+      const double x = sh.red[w];
+      if (!found && x > 0.0) {
+        hit = w;
+        before = run;
+        found = run + x > left;
+      }
+      run += x;
+    }
+    left -= before;
+    const int len = Row<DT, TINY>::run_of(from, to);
+    from += hit * len;
+    to = min(to, from + len);
+    if (to - from <= Row<DT, TINY>::STEP) break;
+  }
+  // at most a step is left (every wave alike)
+  Lane<DT, TINY> a;
+  const int i0 = from + lane * EPL;
+  a.take(Lane<DT, TINY>::raw(row.x, i0, row.n), i0, row.n, to, from + Row<DT, TINY>::STEP);
+  double x[EPL];
+  double sum = 0.0, all;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    x[e] = kept_weight(i0 + e, a.v[e]);
+    sum += x[e];
+  }
+  double run = wave_scan(sum, &all);
+  int hit = 0x7fffffff, lastk = -1;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    run += x[e];
+    if (x[e] > 0.0) {
+      if (run > left) hit = min(hit, i0 + e);
+      lastk = i0 + e;
+    }
+  }
+  hit = wave_min(hit);
+  lastk = wave_max(lastk);
+  return hit != 0x7fffffff ? hit : lastk;
+}
+
+// ---- gather ------------------------------------------------------------------------------------
+// Which maxima bound a row's list: the `k`-th largest of `n` (`fine`: of the quarter groups), n 0
+// for no list. k is top_k, or for nuclei and minima a guess at what they leave.
+struct ListRule {
+  int k, n;
+  bool fine;
+};
+__device__ __forceinline__ ListRule list_rule(const RowSettings& s, int groups) {
+  ListRule r;
+  r.k = s.k > 0 ? s.k : 96;
+  // (with k near the number of maxima the bound falls far below the k-th logit)
+  r.fine = 4 * r.k > 3 * groups;
+  r.n = r.fine ? 4 * groups : groups;
+  if (s.k == 0) r.k = min(r.k, max(1, r.n * 3 / 4));
+  if (r.k > r.n || r.k > kShort) r.n = 0;
+  return r;
+}
+
+// A bound that the k-th largest of n maxima does not fall below, one wave: bisection of the keys'
+// range, the maxima in registers (PER a lane). 20 steps leave a millionth of the range, which costs a
+// few tokens more on the list. -inf where fewer than k are finite.
+template <int PER>
+__device__ __forceinline__ float list_bound(const float* gm, int n, int k) {
+  const int lane = item_id() & 63;
+  const uint32_t none = key_of(kNegInf);
+  uint32_t key[PER], hi = none, least = 0xffffffffu;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int g = 64 * j + lane;
+    key[j] = g < n ? key_of(gm[g]) : none;
+    hi = max(hi, key[j]);
+    least = min(least, key[j] > none ? key[j] : 0xffffffffu);
+  }
+  auto at_least = [&](uint32_t t) {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) c += __popcll(__ballot(key[j] >= t));
+    return c;
+  };
+  if (at_least(none + 1) < k) return kNegInf;
+  // (the signed order of keys with their top bit turned is their own)
+  hi = (uint32_t)wave_max((int)(hi ^ 0x80000000u)) ^ 0x80000000u;
+  uint32_t lo = (uint32_t)wave_min((int)(least ^ 0x80000000u)) ^ 0x80000000u;
+#pragma unroll 1
+  for (int step = 0; step < 20 && lo < hi; ++step) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    if (at_least(mid) >= k) lo = mid;
+    else hi = mid - 1;
+  }
+  return of_key(lo);
+}
+
+template <int DT, bool TINY>
+__global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p, int per) {
+  constexpr int EPL = Lane<DT, TINY>::EPL, IT = kChunk / (256 * EPL);
+  constexpr int kHeld = 1024;  // maxima at most
+  __shared__ float bound;
+  __shared__ int count[2];
+  const int row = wg_id_y(), tid = item_id(), lane = tid & 63;
+  const RowSettings s = settings(p, row);
+  if (s.greedy || !s.filtered()) return;
+  const ListRule rule = list_rule(s, p.groups);
+  const int c0 = wg_id_x() * per, c1 = min(c0 + per, p.chunks);
+  if (rule.n == 0 || rule.n > kHeld) {
+    if (c0 == 0 && tid == 0) p.low[row] = kNegInf;
+    return;
+  }
+  const store_t<DT>* x = reinterpret_cast<const store_t<DT>*>(p.logits) + (int64_t)row * p.ls;
+  u32x4 a[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i)
+    a[i] = Lane<DT, TINY>::raw(x, c0 * kChunk + (i * 256 + tid) * EPL, p.vocab);
+  if (tid < 2) count[tid] = 0;
+  if (tid < 64) {
+    const float* gm = rule.fine ? p.smax + (int64_t)row * p.groups * 4 : p.gmax + (int64_t)row * p.groups;
+    const float b = rule.n <= 128   ? list_bound<2>(gm, rule.n, rule.k)
+                    : rule.n <= 256 ? list_bound<4>(gm, rule.n, rule.k)
+                                    : list_bound<kHeld / 64>(gm, rule.n, rule.k);
+    if (lane == 0) bound = b;
+  }
+  __syncthreads();
+  const float low = bound;
+  if (c0 == 0 && tid == 0) p.low[row] = low;
+  if (low == kNegInf) return;
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    uint64_t* to = p.cand + ((int64_t)row * p.chunks + c) * kShort;
+    int* n = &count[c & 1];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int i0 = c * kChunk + (i * 256 + tid) * EPL;
+      Lane<DT, TINY> cur;
+      cur.take(a[i], i0, p.vocab, p.vocab, c * kChunk + (i + 1) * 256 * EPL);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float l = cur.v[e];
+        const bool take = l >= low;
+        const uint64_t v = __ballot(take);
+        if (v == 0) continue;  // uniform
+        int at = 0;
+        if (lane == 0) at = atomicAdd(n, __popcll(v));
+        at = __builtin_amdgcn_readfirstlane(at) + __popcll(v & ((uint64_t(1) << lane) - 1));
+        if (take && at < kShort) to[at] = rank_of(l, i0 + e);
+      }
+      // the next chunk's loads go out as this one's are done with
+      a[i] = Lane<DT, TINY>::raw(x, i0 + kChunk, p.vocab);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      p.count[(int64_t)row * p.chunks + c] = *n;
+      *n = 0;  // (the next chunk counts in the other word, and its barrier comes before this one's reuse)
+    }
+  }
+}
+
+// ---- pick --------------------------------------------------------------------------------------
+static_assert(kGroup == kPick, "one element of a group per thread");
+
+template <int DT, bool TINY>
 __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) char pick_lds[];
   PickShared& sh = *reinterpret_cast<PickShared*>(pick_lds);
-  const int rowi = wg_id_x(), tid = item_id();
-  Row<DT> row;
+  const int rowi = wg_id_x(), tid = item_id(), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Row<DT, TINY> row;
   row.x = reinterpret_cast<const store_t<DT>*>(p.logits) + (int64_t)rowi * p.ls;
   row.n = p.vocab;
+  row.ring = sh.ring;
   const RowSettings s = settings(p, rowi);
+  const bool simple = s.greedy || !s.filtered();
+  if (s.greedy && wave > 0) return;  // one wave's work, no barrier
   const float uf = p.u[rowi];
   const double u = is_nan(uf) || uf < 0.f ? 0.0 : (double)fminf(uf, 0x1.fffffep-1f);
 
-  // ---- the row's maximum and sums, a thread per chunk
-  const bool on = tid < p.chunks;
-  const int64_t at = (int64_t)rowi * p.chunks + (on ? tid : 0);
-  const f32x4 g = *reinterpret_cast<const f32x4*>(p.gmax + at * 4);
-  const float cm = on ? fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])) : kNegInf;
-  const double ct = p.sum_t[at], c1 = p.sum_1[at];
-  const uint32_t mk = block_reduce_u32(sh, key_of(cm), [](uint32_t a, uint32_t b) { return max(a, b); });
-  const float m = of_key(mk);
+  // ---- the row's maximum, in every wave (lane: groups lane, lane + 64, ..)
+  const int64_t at = (int64_t)rowi * p.groups;
+  const float* gm = p.gmax + at;
+  float m = kNegInf;
+#pragma unroll 2
+  for (int g = lane; g < p.groups; g += 64) m = fmaxf(m, gm[g]);
+  m = wave_max_all(m);
   if (m == kNegInf) {  // nothing to choose from (uniform)
     if (tid == 0) {
       p.tok[rowi] = -1;
@@ -752,187 +1050,157 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     }
     return;
   }
-  const double r1 = block_sum(sh, on ? c1 * weight(cm, m, 1.0) : 0.0);
-  const int first = (int)block_reduce_u32(sh, on && cm == m ? (uint32_t)p.first[at] : 0xffffffffu,
-                                          [](uint32_t a, uint32_t b) { return min(a, b); });
-  int token = first;
-  if (!s.greedy && !s.filtered()) {
-    double w[1] = {on ? ct * weight(cm, m, s.inv) : 0.0};
-    // the chunk, then the token in it by what is left of u W
-    double total;
-    const double before = block_scan(sh, w[0], &total);
-    const int c = draw<1>(sh, w, u);
-    if (tid == c) sh.d[0] = u * total - before;
-    __syncthreads();
-    const double left = sh.d[0];
-    double e[4];
-    const int i0 = c * kChunk + 4 * tid;
-    double mine = 0.0;
+  // log of the row's sum at temperature 1 (m apart), wave 0
+  double logz = 0.0;
+  if (wave == 0 && p.lp) {
+    double r = 0.0;
+#pragma unroll 1
+    for (int g = lane; g < p.groups; g += 64) r += p.sum_1[at + g] * weight(gm[g], m, kLog2e);
+    logz = log(wave_sum(r));
+  }
+  int token = 0;
+  if (s.greedy) {
+    // the first group that holds the maximum, then its first element of that value
+    int g0 = 0x7fffffff;
+#pragma unroll 1
+    for (int g = lane; g < p.groups; g += 64)
+      if (gm[g] == m) g0 = min(g0, g);
+    g0 = wave_min(g0);
+    constexpr int EPL = Row<DT, TINY>::EPL;
+    int f = 0x7fffffff;
+#pragma unroll 1
+    for (int i = g0 * kGroup + (kGroup / 64 - EPL) + kGroup / 64 * lane; i >= g0 * kGroup + kGroup / 64 * lane; i -= EPL) {
+      Lane<DT, TINY> a;
+      a.take(Lane<DT, TINY>::raw(row.x, i, row.n), i, row.n, row.n, (g0 + 1) * kGroup);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      e[j] = i0 + j < row.n ? weight(load1<DT>(row.x, i0 + j), m, s.inv) : 0.0;
-      mine += e[j];
+      for (int e = EPL - 1; e >= 0; --e)
+        if (a.v[e] == m) f = i + e;
     }
-    double run = block_scan(sh, mine, &total);
+    token = wave_min(f);
+  } else if (simple) {
+    // lane: the groups from lane * per; the group that passes u W, then its 1024 elements
+    const int per = (p.groups + 63) / 64, g0 = lane * per;
+    double mine = 0.0, total;
+#pragma unroll 1
+    for (int g = g0; g < min(g0 + per, p.groups); ++g)
+      mine += p.sum_t[at + g] * weight(gm[g], m, s.inv2);
+    double run = wave_scan(mine, &total);
+    const double target = u * total;
+    const uint64_t pass = __ballot(mine > 0.0 && run + mine > target);
+    const uint64_t any = __ballot(mine > 0.0);
+    const int who = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(any);
+    int g_hit = 0;
+    double left = 0.0;
+    if (lane == who) {
+      bool done = false;
+#pragma unroll 1
+      for (int g = g0; g < min(g0 + per, p.groups); ++g) {
+        const double w = p.sum_t[at + g] * weight(gm[g], m, s.inv2);
+        if (!done && w > 0.0) {  // (the last one of any weight where rounding leaves none)
+          g_hit = g;
+          left = target - run;
+          done = run + w > target;
+        }
+        run += w;
+      }
+    }
+    g_hit = __shfl(g_hit, who);
+    left = __shfl(left, who);
+    // the group's elements, one a thread (kGroup == kPick)
+    const int i = g_hit * kGroup + tid;
+    const double w = i < row.n ? weight(load1<DT>(row.x, i), m, s.inv2) : 0.0;
+    run = block_scan(sh, w, &total);
     if (tid == 0) {
       sh.i[0] = 0x7fffffff;
       sh.i[1] = 0;
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      run += e[j];
-      if (e[j] > 0.0) {
-        if (run > left) atomicMin(&sh.i[0], i0 + j);
-        atomicMax(&sh.i[1], i0 + j);
-      }
+    const int hit = wave_min(w > 0.0 && run + w > left ? i : 0x7fffffff);
+    const int lastk = wave_max(w > 0.0 ? i : 0);
+    if (lane == 0) {
+      atomicMin(&sh.i[0], hit);
+      atomicMax(&sh.i[1], lastk);
     }
     __syncthreads();
     token = sh.i[0] != 0x7fffffff ? sh.i[0] : sh.i[1];
-  } else if (!s.greedy) {
-    const double W = s.k == 0 ? block_sum(sh, on ? ct * weight(cm, m, s.inv) : 0.0) : 0.0;
-    // ---- a list of everything from the k-th largest group maximum up
-    const int groups = 4 * p.chunks;
-    const int k = s.k > 0 ? s.k : min(groups, 96);
-    bool done = false;
-    if (k <= groups && groups <= kList) {
-      __syncthreads();
-      if (on)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sh.sorted[4 * tid + e] = rank_of(g[e], 4 * tid + e);
-      __syncthreads();
-      sort_list(sh, groups);
-      const float low = logit_of(sh.sorted[k - 1]);
-      if (low != kNegInf) {
-        const int n = collect(row, sh, [&](int, float l) { return l >= low; });
-        if (n <= kList) {
-          // every kept token is listed when the k-th, the least weight or the limit ends inside
-          const bool by_mp = s.mp > 0.0 && weight(low, m, s.inv) < s.mp;
-          double whole = -1.0;
-          done = s.k > 0 || by_mp;
-          if (!done && s.mp <= 0.0 && s.p < 1.f) {
-            double x = 0.0;
-            for (int j = tid; j < n; j += kPick) x += weight(logit_of(sh.list[j]), m, s.inv);
-            x = block_sum(sh, x);
-            // (a limit so near the list's end that rounding decides goes to the general way)
-            done = x * (1.0 - 1e-12) >= (double)s.p * W;
-            whole = W;
-          }
-          if (done) token = pick_from_list(sh, n, s, m, whole, u);
-        }
-      }
-    }
-    if (!done) {
-      // ---- the general way
-      Kept kept = {0, s.mp};
-      if (s.k > 0) kept.low = boundary(row, sh, m, s.inv, Kept{0, 0.0}, true, s.k, 0.0);
-      if (s.p < 1.f) {
-        double w1 = W;
-        if (s.k > 0 || s.mp > 0.0) {
-          w1 = 0.0;
-          row.each([&](int i, float l) {
-            if (l == kNegInf || rank_of(l, i) < kept.low) return;
-            const double w = weight(l, m, s.inv);
-            if (w >= kept.mp) w1 += w;
-          });
-          w1 = block_sum(sh, w1);
-        }
-        // (a limit of 0 or less keeps the first alone)
-        kept.low = boundary(row, sh, m, s.inv, kept, false, 0, (double)s.p * w1);
-      }
-      // sums of the kept weights by segments in index order: a wave's share of a tile
-      constexpr int EPL = Row<DT>::EPL, TILE = Row<DT>::TILE, SEG = 64 * EPL;
-      auto kept_weight = [&](int i, float l) {
-        if (l == kNegInf || rank_of(l, i) < kept.low) return 0.0;
-        const double w = weight(l, m, s.inv);
-        return w >= kept.mp ? w : 0.0;
-      };
-      const int segs = (row.n + SEG - 1) / SEG;
-      __syncthreads();
+  } else {
+    double W = 0.0;
+    if (s.k == 0) {
 #pragma unroll 1
-      for (int b = tid * EPL; b < (row.n + TILE - 1) / TILE * TILE; b += TILE) {
-        Lane<DT> a;
-        a.load(row.x, min(b, row.n), row.n);
-        double x = 0.0;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) x += kept_weight(b + e, a.v[e]);
-        x = wave_sum(x);
-        if ((tid & 63) == 0 && b / SEG < segs) sh.seg[b / SEG] = x;
-      }
-      __syncthreads();
-      double w[4];
-      double mine = 0.0, total;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[e] = 4 * tid + e < segs ? sh.seg[4 * tid + e] : 0.0;
-        mine += w[e];
-      }
-      double before = block_scan(sh, mine, &total);
-      const int sg = draw<4>(sh, w, u);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (4 * tid + e == sg) sh.d[0] = u * total - before;
-        before += w[e];
-      }
-      __syncthreads();
-      const double left = sh.d[0];
-      // the segment, one wave
-      if (tid < 64) {
-        Lane<DT> a;
-        const int i0 = sg * SEG + tid * EPL;
-        a.load(row.x, min(i0, row.n), row.n);
-        double x[EPL];
-        double sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-          x[e] = kept_weight(i0 + e, a.v[e]);
-          sum += x[e];
-        }
-        double inc = sum;
+      for (int g = lane; g < p.groups; g += 64) W += p.sum_t[at + g] * weight(gm[g], m, s.inv2);
+      W = wave_sum(W);
+    }
+    // ---- the gathered list (the rule that made it says whether there is one)
+    bool done = false;
+    const ListRule rule = list_rule(s, p.groups);
+    const float low = rule.n == 0 ? kNegInf : p.low[rowi];
+    if (low != kNegInf) {
+      // chunk counts by lane (every wave alike), places by their running sum
+      const int32_t* counts = p.count + (int64_t)rowi * p.chunks;
+      int n = 0;
+      for (int c0 = 0; c0 < p.chunks; c0 += 64) {
+        const int c = c0 + lane < p.chunks ? counts[c0 + lane] : 0;
+        int before = c;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-          const double y = __shfl_up(inc, d);
-          if (tid >= d) inc += y;
+          const int y = __shfl_up(before, d);
+          if (lane >= d) before += y;
         }
-        double run = __shfl_up(inc, 1);
-        if (tid == 0) run = 0.0;
-        int hit = 0x7fffffff, lastk = -1;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-          run += x[e];
-          if (x[e] > 0.0) {
-            if (run > left) hit = min(hit, i0 + e);
-            lastk = i0 + e;
-          }
+        const int all = __shfl(before, 63);
+        before += n - c;
+        // waves take the chunks in turn
+        for (int j = wave; j < min(64, p.chunks - c0); j += kWaves) {
+          const int cj = min(__shfl(c, j), kShort), at0 = __shfl(before, j);
+          const uint64_t* from = p.cand + ((int64_t)rowi * p.chunks + c0 + j) * kShort;
+          for (int q = lane; q < cj; q += 64)
+            if (at0 + q < kShort) sh.raw[at0 + q] = from[q];
         }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          hit = min(hit, __shfl_xor(hit, d));
-          lastk = max(lastk, __shfl_xor(lastk, d));
+        n += all;
+      }
+      __syncthreads();
+      if (n <= kShort) {
+        // every kept token is listed when the k-th, the least weight or the limit ends inside
+        const bool by_mp = s.mp > 0.0 && weight(low, m, s.inv2) < s.mp;
+        double whole = -1.0;
+        done = s.k > 0 || by_mp;
+        if (!done && s.mp <= 0.0 && s.p < 1.f) {
+          double x = tid < n ? weight(logit_of(sh.raw[tid]), m, s.inv2) : 0.0;
+          x = block_sum(sh, x);
+          // (a limit so near the list's end that rounding decides goes the wide way)
+          done = x * (1.0 - 1e-12) >= (double)s.p * W;
+          whole = W;
         }
-        token = hit != 0x7fffffff ? hit : lastk;
+        if (done) token = pick_short(sh, n, s, m, whole, u);
       }
     }
+    if (!done) token = pick_wide(row, sh, s, m, W, u);
   }
   if (tid == 0) {
     p.tok[rowi] = token;
     if (p.lp) {
       const float l = load1<DT>(row.x, token);
       const double d = l >= m ? 0.0 : (double)l - (double)m;
-      p.lp[rowi] = (float)(d - log(r1));
+      p.lp[rowi] = (float)(d - logz);
     }
   }
 }
 
-template <int DT>
+template <int DT, bool TINY>
 hipError_t launch_sample(const SampleParams& p, hipStream_t st) {
   static const hipError_t once = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(sample_pick_kernel<DT>),
+      reinterpret_cast<const void*>(sample_pick_kernel<DT, TINY>),
       hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PickShared));
   if (once != hipSuccess) return once;
-  hipLaunchKernelGGL(sample_scan_kernel<DT>, dim3((unsigned)p.chunks, (unsigned)p.rows), dim3(256), 0,
+  hipLaunchKernelGGL((sample_scan_kernel<DT, TINY>), dim3((unsigned)((p.groups + 3) / 4), (unsigned)p.rows), dim3(256), 0,
                      st, p);
-  hipLaunchKernelGGL(sample_pick_kernel<DT>, dim3((unsigned)p.rows), dim3(kPick), sizeof(PickShared),
+  if (p.k || p.k_all > 0 || p.p || p.p_all < 1.f || p.mp || p.mp_all > 0.f) {  // a row may filter
+    // four chunks a workgroup where that leaves enough of them: each finds the row's bound by itself
+    const int per = (int64_t)p.chunks * p.rows >= 4096 ? 4 : 1;
+    hipLaunchKernelGGL((sample_gather_kernel<DT, TINY>),
+                       dim3((unsigned)((p.chunks + per - 1) / per), (unsigned)p.rows), dim3(256), 0,
+                       st, p, per);
+  }
+  hipLaunchKernelGGL((sample_pick_kernel<DT, TINY>), dim3((unsigned)p.rows), dim3(kPick), sizeof(PickShared),
                      st, p);
   return hipGetLastError();
 }
@@ -942,9 +1210,27 @@ int check_sample_sizes(int32_t rows, int32_t vocab) {
   if (vocab < 1 || vocab > kMaxVocab) return api_fail(FFAI_ERR_INVALID, "vocab must be in [1, 2^20]");
   return FFAI_OK;
 }
-size_t sample_bytes(int32_t rows, int32_t vocab) {
-  const size_t n = (size_t)rows * ((vocab + kChunk - 1) / kChunk);
-  return n * (16 + 8 + 8) + ((n * 4 + 15) & ~size_t(15));
+// The workspace's parts, in order, each 16-byte aligned.
+struct SampleSpace {
+  size_t sum_t, sum_1, cand, gmax, smax, low, count, bytes;
+};
+SampleSpace sample_space(int32_t rows, int32_t vocab) {
+  const size_t g = (size_t)rows * ((vocab + kGroup - 1) / kGroup);
+  const size_t c = (size_t)rows * ((vocab + kChunk - 1) / kChunk);
+  SampleSpace s{};
+  auto take = [&](size_t n) {
+    const size_t at = s.bytes;
+    s.bytes += (n + 15) & ~size_t(15);
+    return at;
+  };
+  s.sum_t = take(g * 8);
+  s.sum_1 = take(g * 8);
+  s.cand = take(c * kShort * 8);
+  s.gmax = take(g * 4);
+  s.smax = take(g * 16);
+  s.low = take((size_t)rows * 4);
+  s.count = take(c * 4);
+  return s;
 }
 
 }  // namespace
@@ -959,7 +1245,7 @@ int ffai_sample_workspace_bytes(int32_t rows, int32_t vocab, size_t* bytes) {
   if (!bytes) return api_fail(FFAI_ERR_INVALID, "null bytes pointer");
   const int rc = check_sample_sizes(rows, vocab);
   if (rc != FFAI_OK) return rc;
-  *bytes = sample_bytes(rows, vocab);
+  *bytes = sample_space(rows, vocab).bytes;
   return FFAI_OK;
 }
 
@@ -982,29 +1268,38 @@ int ffai_sample(const void* logits, int32_t logits_dtype, int32_t rows, int32_t 
     return api_fail(FFAI_ERR_INVALID, "settings, u and outputs must be 4-byte aligned");
   if (logits_row_stride < 0)
     return api_fail(FFAI_ERR_INVALID, "logits row stride must not be negative");
-  if (!workspace || workspace_bytes < sample_bytes(rows, vocab))
+  if (!workspace || workspace_bytes < sample_space(rows, vocab).bytes)
     return api_fail(FFAI_ERR_WORKSPACE, "workspace smaller than ffai_sample_workspace_bytes");
   if ((uintptr_t)workspace % 16) return api_fail(FFAI_ERR_INVALID, "workspace must be 16-byte aligned");
   rc = api_check_device();
   if (rc != FFAI_OK) return rc;
   SampleParams p{};
   p.logits = logits; p.ls = logits_row_stride; p.rows = rows; p.vocab = vocab;
-  p.chunks = (vocab + kChunk - 1) / kChunk;
+  p.groups = (vocab + kGroup - 1) / kGroup;
   p.t = temperature; p.t_all = temperature_all;
   p.k = top_k; p.k_all = top_k_all;
   p.p = top_p; p.p_all = top_p_all;
   p.mp = min_p; p.mp_all = min_p_all;
   p.u = u; p.tok = tokens; p.lp = logprobs;
-  const size_t n = (size_t)rows * p.chunks;
+  p.chunks = (vocab + kChunk - 1) / kChunk;
+  const SampleSpace sp = sample_space(rows, vocab);
   char* ws = static_cast<char*>(workspace);
-  p.gmax = reinterpret_cast<float*>(ws);
-  p.sum_t = reinterpret_cast<double*>(ws + n * 16);
-  p.sum_1 = reinterpret_cast<double*>(ws + n * 24);
-  p.first = reinterpret_cast<int32_t*>(ws + n * 32);
+  p.sum_t = reinterpret_cast<double*>(ws + sp.sum_t);
+  p.sum_1 = reinterpret_cast<double*>(ws + sp.sum_1);
+  p.cand = reinterpret_cast<uint64_t*>(ws + sp.cand);
+  p.gmax = reinterpret_cast<float*>(ws + sp.gmax);
+  p.smax = reinterpret_cast<float*>(ws + sp.smax);
+  p.low = reinterpret_cast<float*>(ws + sp.low);
+  p.count = reinterpret_cast<int32_t*>(ws + sp.count);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const hipError_t e = logits_dtype == FFAI_F32   ? launch_sample<kF32>(p, st)
-                       : logits_dtype == FFAI_F16 ? launch_sample<kF16>(p, st)
-                                                  : launch_sample<kBF16>(p, st);
+  const bool tiny = vocab < (logits_dtype == FFAI_F32 ? 4 : 8);  // less than a lane's load
+  auto launch = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    return tiny ? launch_sample<DT, true>(p, st) : launch_sample<DT, false>(p, st);
+  };
+  const hipError_t e = logits_dtype == FFAI_F32   ? launch(std::integral_constant<int, kF32>{})
+                       : logits_dtype == FFAI_F16 ? launch(std::integral_constant<int, kF16>{})
+                                                  : launch(std::integral_constant<int, kBF16>{});
   if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));
   return FFAI_OK;
 }

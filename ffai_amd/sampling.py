@@ -7,6 +7,8 @@ uniform numbers, and the token's log-probability. The header says exactly which 
 
 from __future__ import annotations
 
+import ctypes
+import functools
 from typing import Optional, Union
 
 import torch
@@ -15,12 +17,10 @@ from . import _lib as L
 from .flash_attn import _DT
 
 Setting = Union[None, float, int, torch.Tensor]
-_CHUNK = 4096  # logits of one scan workgroup (what workspace_bytes is counted in)
 
 
+@functools.lru_cache(maxsize=256)
 def workspace_bytes(rows: int, vocab: int) -> int:
-    import ctypes
-
     n = ctypes.c_size_t(0)
     L.check(L.load().ffai_sample_workspace_bytes(rows, vocab, ctypes.byref(n)))
     return n.value
@@ -67,9 +67,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = None
             raise ValueError(f"out must be a contiguous int32 tensor of {rows} on {device}")
         lp = torch.empty(rows, dtype=torch.float32, device=device) if logprobs else None
         if workspace is None:
-            n = rows * -(-vocab // _CHUNK)
-            workspace = torch.empty(n * 32 + (n * 4 + 15) // 16 * 16, dtype=torch.uint8,
-                                    device=device)
+            workspace = torch.empty(workspace_bytes(rows, vocab), dtype=torch.uint8, device=device)
         elif workspace.device != device or not workspace.is_contiguous():
             raise ValueError(f"workspace must be contiguous, on {device}")
         L.check(L.load().ffai_sample(

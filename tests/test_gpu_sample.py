@@ -53,7 +53,7 @@ def make(gpu, rows, vocab, sigma=2.5, seed=0, dtype=torch.float32, low=0.03):
     return l.to(dtype).to(gpu), torch.rand(rows, generator=g).to(gpu)
 
 
-VOCABS = [1, 2, 3, 63, 1000, 4095, 4096, 4097, 8193, 51865]
+VOCABS = [1, 2, 3, 4, 5, 7, 8, 9, 63, 1000, 4095, 4096, 4097, 8193, 51865]
 
 
 @pytest.mark.parametrize("vocab", VOCABS)

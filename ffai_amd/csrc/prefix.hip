@@ -125,29 +125,57 @@ int check_sizes(const ffai_kv_cache* pre, const ffai_kv_cache* own, int32_t head
 
 struct PrefixPlan {
   int R, M, pieces_p, pieces_o, blocks_p, blocks_o;
+  bool many;
+  int block_slots;  // > 0: the whole attention in one launch, this many slots a workgroup
   int64_t items_p, items_o, rows;
   size_t part_bytes, bytes;
 };
+
+constexpr int64_t kWholeTiles = 40;
 
 PrefixPlan plan_prefix(const ffai_kv_cache* pre, const ffai_kv_cache* own, int heads_q, int q_len) {
   PrefixPlan p{};
   p.R = heads_q / own->heads * q_len;
   p.M = own->slots / pre->slots * p.R;
-  p.blocks_p = (p.M + kPrefixRowBlock - 1) / kPrefixRowBlock;
-  p.blocks_o = (p.R + kPrefixRowBlock - 1) / kPrefixRowBlock;
+  const int block = prefix_row_block(own->head_dim);
+  const int64_t units = (int64_t)pre->slots * own->heads;
+  const int64_t units_o = (int64_t)own->slots * own->heads * ((p.R + block - 1) / block);
+  const int64_t tiles_p = (pre->capacity + kBlockN - 1) / kBlockN;
+  const int64_t tiles_o = (own->capacity + kBlockN - 1) / kBlockN;
+  auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  // Few tiles for a block of whole slots: one launch, no partials (the launch and the round trip of a
+  // merge cost as much as the attention of a short step).
+  if (p.R <= block) {
+    const int64_t per = own->slots / pre->slots;
+    const int64_t bs = std::min<int64_t>(per, block / p.R);
+    if (tiles_p + bs * tiles_o <= kWholeTiles) {
+      p.block_slots = (int)bs;
+      p.blocks_p = (int)ceil_div(per, bs);
+      p.pieces_p = 1;
+      p.items_p = (int64_t)pre->slots * own->heads * p.blocks_p;
+      p.rows = (int64_t)own->slots * heads_q * q_len;
+      return p;
+    }
+  }
+  // Row blocks of 32 or 16 read the prefix once each, through the caches, and their waves run a tile's
+  // whole chain alone: short, but far from the matrix cores' rate. Blocks of 128 share a tile among
+  // four waves; they pay off once the products outweigh the chain.
+  const int64_t wave_tiles = units * ceil_div(p.M, 32) * tiles_p;
+  p.many = p.M > 64 && wave_tiles >= 4096;
+  p.blocks_p = (int)ceil_div(p.M, p.many ? kPrefixManyRows : block);
+  p.blocks_o = (p.R + block - 1) / block;
+  const int64_t units_p = units * p.blocks_p;
   // Key pieces: enough workgroups for two on every CU, but no fewer than four tiles (one a wave)
-  // to a piece, since every piece of a row is written once and read once by the merge.
-  const int64_t units_p = (int64_t)pre->slots * own->heads * p.blocks_p;
-  const int64_t units_o = (int64_t)own->slots * own->heads * p.blocks_o;
-  const int64_t most_p = (pre->capacity + 4 * kBlockN - 1) / (4 * kBlockN);
-  const int64_t most_o = (own->capacity + 4 * kBlockN - 1) / (4 * kBlockN);
+  // to a piece, since every piece of a row is written once and read once by the merge. Blocks of
+  // 128 rows: one workgroup on every CU beside the own pieces, eight tiles at least.
   constexpr int64_t kTarget = 512;
-  auto pieces = [&](int64_t most, int64_t units, int64_t others) {
-    return (int)std::min<int64_t>(std::min<int64_t>(most, 64),
-                                  std::max<int64_t>(1, (kTarget - others + units - 1) / units));
+  auto pieces = [&](int64_t tiles, int64_t least, int64_t target, int64_t n) {
+    return (int)std::min<int64_t>(std::min<int64_t>(ceil_div(tiles, least), 64),
+                                  std::max<int64_t>(1, ceil_div(target, n)));
   };
-  p.pieces_p = pieces(most_p, units_p, units_o);
-  p.pieces_o = pieces(most_o, units_o, units_p * p.pieces_p);
+  p.pieces_p = p.many ? pieces(tiles_p, 8, kTarget, units_p)
+                      : pieces(tiles_p, 4, std::max<int64_t>(kTarget - units_o, kTarget / 2), units_p);
+  p.pieces_o = pieces(tiles_o, 4, kTarget - (p.many ? 0 : units_p * p.pieces_p), units_o);
   p.items_p = units_p * p.pieces_p;
   p.items_o = units_o * p.pieces_o;
   p.rows = (int64_t)own->slots * heads_q * q_len;
@@ -196,7 +224,7 @@ int ffai_prefix_attn_plan_info(const ffai_kv_cache* prefix, const ffai_kv_cache*
   info[1] = p.pieces_p;
   info[2] = p.pieces_o;
   info[3] = (int32_t)(p.items_p + p.items_o);
-  info[4] = std::min(p.M, kPrefixRowBlock);
+  info[4] = p.block_slots > 0 ? p.block_slots * p.R : std::min(p.M, p.many ? kPrefixManyRows : prefix_row_block(own->head_dim));
   return FFAI_OK;
 }
 
@@ -233,7 +261,7 @@ int ffai_prefix_attn_fwd(const ffai_kv_cache* prefix, const ffai_kv_cache* own, 
   const PrefixPlan pl = plan_prefix(prefix, own, heads_q, q_len);
   if (pl.items_p + pl.items_o > 0x7fffffff)
     return api_fail(FFAI_ERR_INVALID, "problem too large");
-  if (!workspace || workspace_bytes < pl.bytes)
+  if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes))
     return api_fail(FFAI_ERR_WORKSPACE, "workspace smaller than ffai_prefix_attn_workspace_bytes");
   if ((uintptr_t)workspace % 16)
     return api_fail(FFAI_ERR_INVALID, "workspace must be 16-byte aligned");
@@ -243,7 +271,8 @@ int ffai_prefix_attn_fwd(const ffai_kv_cache* prefix, const ffai_kv_cache* own, 
   PrefixParams p{};
   p.q = q;
   p.q_ss = q_strides[0]; p.q_sh = q_strides[1]; p.q_st = q_strides[2];
-  p.q_f32 = q_dtype == FFAI_F32;
+  p.out = out;
+  p.o_ss = o_strides[0]; p.o_sh = o_strides[1]; p.o_st = o_strides[2];
   auto side = [](const ffai_kv_cache* c, int pieces, int blocks, int64_t items) {
     PrefixSide s{};
     s.k = c->k; s.v = c->v; s.lens = c->lens;
@@ -257,11 +286,25 @@ int ffai_prefix_attn_fwd(const ffai_kv_cache* prefix, const ffai_kv_cache* own, 
   p.ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.part_bytes);
   p.per = own->slots / prefix->slots;
   p.Hkv = own->heads; p.rep = heads_q / own->heads; p.T = q_len; p.R = pl.R; p.M = pl.M;
+  p.many = pl.many;
+  p.stride = getenv("PSTRIDE") ? (pl.many ? (int32_t)std::min<int64_t>(1 + pl.items_o / pl.items_p, 1 << 20) : 0) : 0;
   p.scale_log2 = scale * 1.44269504088896340736f;
   const int parts = q_dtype == FFAI_F32     ? kPartsBoth
                     : out_dtype == FFAI_F32 ? kPartsWeights
                                             : kPartsOne;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (pl.block_slots > 0) {
+    p.block_slots = pl.block_slots;
+    if (parts == kPartsBoth && p.R <= 16) {  // (an f32 q's parts leave registers for 16 rows)
+      p.block_slots = std::min(p.per, 16 / p.R);
+      p.pre.row_blocks = (p.per + p.block_slots - 1) / p.block_slots;
+    }
+    const hipError_t e = dt == FFAI_F16
+                             ? launch_whole_f16(p, prefix->slots, own->head_dim, parts, st)
+                             : launch_whole_bf16(p, prefix->slots, own->head_dim, parts, st);
+    if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));
+    return FFAI_OK;
+  }
   hipError_t e = dt == FFAI_F16 ? launch_prefix_f16(p, own->head_dim, parts, st)
                                 : launch_prefix_bf16(p, own->head_dim, parts, st);
   if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));

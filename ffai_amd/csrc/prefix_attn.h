@@ -21,7 +21,8 @@ struct PrefixSide {
 struct PrefixParams {
   const void* q;
   int64_t q_ss, q_sh, q_st;  // slot, head, row strides (elements)
-  int32_t q_f32;
+  void* out;  // prefix_whole_kernel writes it; else the merge does
+  int64_t o_ss, o_sh, o_st;
   PrefixSide pre, own;
   float* part;  // partial rows: O [row][piece][D], row = (slot * Hkv + head) * R + rr, pieces of
                 // the prefix first, then the own ones
@@ -30,6 +31,9 @@ struct PrefixParams {
   int32_t Hkv, rep, T;
   int32_t R;  // rows of a slot that read one K/V head: rep * T
   int32_t M;  // rows of a group that read one prefix K/V head: per * R
+  int32_t block_slots;  // prefix_whole_kernel: slots of a workgroup
+  int32_t many;    // the prefix's pieces in blocks of kPrefixManyRows rows (prefix_rows)
+  int32_t stride;  // then: every stride-th item of the grid's first ones is a prefix piece
   float scale_log2;
 };
 
@@ -52,8 +56,15 @@ enum PrefixParts : int {
 
 hipError_t launch_prefix_f16(const PrefixParams& p, int head_dim, int parts, hipStream_t s);
 hipError_t launch_prefix_bf16(const PrefixParams& p, int head_dim, int parts, hipStream_t s);
+// The whole attention in one launch (p.block_slots, p.pre.row_blocks set; no workspace).
+hipError_t launch_whole_f16(const PrefixParams& p, int groups, int head_dim, int parts, hipStream_t s);
+hipError_t launch_whole_bf16(const PrefixParams& p, int groups, int head_dim, int parts, hipStream_t s);
 
 constexpr int kPrefixWaves = 4;     // waves of a workgroup, a key tile each
-constexpr int kPrefixRowBlock = 32;  // rows of a workgroup: two 16-column MFMA blocks
+// Rows of a workgroup of prefix_work: two 16-column MFMA blocks at head_dim 64. At 128 one: two need
+// more than the 256 registers that leave room for two workgroups on a CU.
+constexpr int prefix_row_block(int head_dim) { return head_dim == 64 ? 32 : 16; }
+constexpr int kWholeWaves = 8;  // waves of a workgroup of prefix_whole_kernel
+constexpr int kPrefixManyRows = 128;  // rows of a workgroup of prefix_rows: 32 a wave
 
 }  // namespace ffai

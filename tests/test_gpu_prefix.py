@@ -97,13 +97,55 @@ SHAPES = {
 
 @pytest.mark.parametrize("shape", SHAPES, ids=[s.replace(" ", "_") for s in SHAPES])
 @pytest.mark.parametrize("io", IO, ids=["-".join(i) for i in IO])
-def test_against_the_definition(gpu, shape, io):
+@pytest.mark.parametrize("roomy", [False, True], ids=["tight", "roomy"])
+def test_against_the_definition(gpu, shape, io, roomy):
+    """`roomy`: the same sequences in caches of a large capacity, which run in pieces with a merge
+    where the tight ones run in one launch."""
     q, kv, out = io
     gr, per, hkv, rep, t, d, pl, ol, pc, oc = SHAPES[shape]
+    if roomy:
+        pc, pl = pc + 3000, [min(n, pc) for n in pl]  # (a length past the tight capacity ends there)
+        oc, ol = oc + 3000, [min(n, oc) for n in ol]
     x = make(gpu, gr, per, hkv, rep, t, d, pl, ol, pc, oc, q, kv)
     got = prefix_attention(x["q"], *caches(x), scale=d ** -0.5, out_dtype=DT[out])
     assert got.dtype == DT[out] and got.shape == x["q"].shape
     check(got, x, d ** -0.5, DT[out])
+
+
+# shapes whose prefix runs in shared tiles (blocks of 128 rows): a block with an idle wave, ragged
+# blocks, one query token and several, groups of unlike lengths, one empty
+MANY = {
+    "an idle wave": (1, 70, 16, 1, 1, 64, [5600], list(range(1, 71)), 5601, 72),
+    "ragged blocks, grouped": (1, 50, 4, 4, 1, 128, [9500], list(range(70, 120)), 9600, 120),
+    "tokens and groups": (4, 10, 4, 3, 3, 128, [5700, 0, 64, 5631], [3 + i for i in range(40)], 5700, 44),
+}
+
+
+@pytest.mark.parametrize("shape", MANY, ids=[s.replace(" ", "_") for s in MANY])
+@pytest.mark.parametrize("io", [IO[0], IO[1], IO[2], IO[5]], ids=lambda i: "-".join(i))
+def test_many_rows(gpu, shape, io):
+    q, kv, out = io
+    gr, per, hkv, rep, t, d, pl, ol, pc, oc = MANY[shape]
+    x = make(gpu, gr, per, hkv, rep, t, d, pl, ol, pc, oc, q, kv, seed=19)
+    plan = PrefixAttention(*caches(x), hkv * rep, t, q_dtype=DT[q], out_dtype=DT[out], scale=d ** -0.5)
+    assert plan.plan()["row_block"] > 32
+    got = plan(x["q"])
+    check(got, x, d ** -0.5, DT[out])
+    assert torch.equal(got, plan(x["q"]))
+
+
+@pytest.mark.parametrize("cap", [80, 4000])
+def test_one_slots_infinities_stay_its_own(gpu, cap):
+    """One query token a slot: a slot whose every V is infinite or NaN among ordinary ones."""
+    x = make(gpu, 1, 5, 2, 1, 1, 64, [70], [66, 40, 3, 0, 80], 70, cap, "bf16", "bf16", seed=6)
+    x["ov"][1, :, 3] = float("inf")
+    x["ov"][2, 0, 1, 3] = float("nan")
+    x["ok"][4, 1, 7] = float("nan")
+    got = prefix_attention(x["q"], *caches(x), scale=0.125)
+    check(got, x, 0.125, torch.bfloat16)
+    assert torch.isfinite(got[[0, 3]]).all() and torch.isinf(got[1]).all()
+    assert torch.isnan(got[2, 0, 0, 3]) and torch.isfinite(got[2, 1]).all()
+    assert torch.isnan(got[4, 1]).all() and torch.isfinite(got[4, 0]).all()
 
 
 @pytest.mark.parametrize("kv", ["bf16", "f16"])
@@ -116,10 +158,12 @@ def test_flat_and_sharp_rows(gpu, kv, gain):
 
 
 @pytest.mark.parametrize("io", [("f16", "f16", "f16"), ("f32", "bf16", "f32")])
-def test_non_finite_values_of_keys_that_a_row_does_not_see(gpu, io):
-    """A later token's K and V may hold anything: only the rows that see it are touched."""
+@pytest.mark.parametrize("cap", [66, 4000])
+def test_non_finite_values_of_keys_that_a_row_does_not_see(gpu, io, cap):
+    """A later token's K and V may hold anything, and so may another slot's: only the rows that see
+    them are touched."""
     q, kv, out = io
-    x = make(gpu, 1, 2, 1, 2, 4, 64, [70], [66, 40], 70, 66, q, kv, seed=5)
+    x = make(gpu, 1, 2, 1, 2, 4, 64, [70], [66, 40], 70, cap, q, kv, seed=5)
     x["ok"][0, :, 64] = float("nan")
     x["ov"][0, :, 65, 5] = float("inf")
     x["ov"][1, :, 39, 7] = float("nan")
@@ -264,7 +308,8 @@ def test_shared_output_of_a_plan(gpu):
 
 
 def test_a_short_workspace_is_refused(gpu):
-    x = make(gpu, 1, 2, 1, 1, 1, 64, [20], [5, 9], 20, 12)
+    x = make(gpu, 1, 2, 1, 1, 1, 64, [3000], [5, 9], 3000, 12)
     plan = PrefixAttention(*caches(x), 1)
+    plan(x["q"], workspace=torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=gpu))
     with pytest.raises(L.FfaiError, match="workspace"):
         plan(x["q"], workspace=torch.empty(plan.workspace_bytes - 1, dtype=torch.uint8, device=gpu))

@@ -67,7 +67,7 @@ def test_bad_arguments(edit, why):
 
 def test_workspace_is_checked():
     for ws in (dict(ws=0), dict(ws_bytes=0)):
-        rc, msg = fwd(cache(2), cache(4), **ws)
+        rc, msg = fwd(cache(2, cap=4000), cache(4), **ws)
         assert rc == L.FFAI_ERR_WORKSPACE and "workspace" in msg
 
 
@@ -129,16 +129,28 @@ def test_from_tensors_views_what_it_is_given():
 @pytest.mark.parametrize("groups,per,hkv,rep,t,pcap,ocap", [
     (1, 1, 1, 1, 1, 1, 1), (1, 5, 16, 1, 1, 37, 448), (8, 5, 16, 1, 1, 224, 224),
     (1, 16, 2, 6, 1, 4096, 512), (1, 128, 8, 4, 1, 16384, 1024), (3, 8, 20, 1, 5, 1111, 400),
-    (1, 1, 1, 8, 7, 100000, 3)])
-def test_plan_covers_every_key_and_row(groups, per, hkv, rep, t, pcap, ocap):
-    """Pieces of whole tiles, at least one a side and at most one per four tiles, and a workspace
-    that holds every piece of every row."""
-    pre, own = cache(groups, hkv, pcap), cache(groups * per, hkv, ocap)
+    (1, 1, 1, 8, 7, 100000, 3), (1, 1, 1, 40, 1, 10, 10)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_plan_covers_every_key_and_row(groups, per, hkv, rep, t, pcap, ocap, d):
+    """One launch over whole slots with no workspace; or pieces of whole tiles, at least one a side
+    and at most one per four tiles, and a workspace that holds every piece of every row."""
+    pre, own = cache(groups, hkv, pcap, d), cache(groups * per, hkv, ocap, d)
     plan = PrefixAttention(pre, own, hkv * rep, t)
     p = plan.plan()
     assert p["rows"] == per * rep * t
+    assert 1 <= p["row_block"] <= 128
+    if plan.workspace_bytes == 0:
+        slots = p["row_block"] // (rep * t)
+        assert slots >= 1 and p["own_pieces"] == 0
+        assert p["workgroups"] == groups * hkv * -(-per // slots)
+        return
     assert 1 <= p["prefix_pieces"] <= max(1, -(-pcap // 256))
     assert 1 <= p["own_pieces"] <= max(1, -(-ocap // 256))
     rows = groups * per * hkv * rep * t
     pieces = p["prefix_pieces"] + p["own_pieces"]
-    assert plan.workspace_bytes >= rows * pieces * (64 + 2) * 4
+    assert plan.workspace_bytes >= rows * pieces * (d + 2) * 4
+
+
+def test_short_sequences_take_no_workspace():
+    assert PrefixAttention(cache(1, 16, 37), cache(5, 16, 448), 16).workspace_bytes == 0
+    assert PrefixAttention(cache(1, 16, 4096), cache(5, 16, 448), 16).workspace_bytes > 0

@@ -131,6 +131,10 @@ struct PrefixPlan {
   size_t part_bytes, bytes;
 };
 
+// By capacity, which is what the host knows: five rounds of a workgroup's eight waves. 5 beams x 16
+// heads, 37 shared and 40 own keys of capacity 448: 5.8 us (7.05 in two launches), 8 x 5 beams x 16
+// heads, 224 shared and 200 own keys (24 tiles) with an f32 result 11.5 (13.2); head_dim 128, 8 x 16
+// slots x 32 heads, 128 and 128 keys 18.3 (23.1).
 constexpr int64_t kWholeTiles = 40;
 
 PrefixPlan plan_prefix(const ffai_kv_cache* pre, const ffai_kv_cache* own, int heads_q, int q_len) {
@@ -287,7 +291,6 @@ int ffai_prefix_attn_fwd(const ffai_kv_cache* prefix, const ffai_kv_cache* own, 
   p.per = own->slots / prefix->slots;
   p.Hkv = own->heads; p.rep = heads_q / own->heads; p.T = q_len; p.R = pl.R; p.M = pl.M;
   p.many = pl.many;
-  p.stride = getenv("PSTRIDE") ? (pl.many ? (int32_t)std::min<int64_t>(1 + pl.items_o / pl.items_p, 1 << 20) : 0) : 0;
   p.scale_log2 = scale * 1.44269504088896340736f;
   const int parts = q_dtype == FFAI_F32     ? kPartsBoth
                     : out_dtype == FFAI_F32 ? kPartsWeights
@@ -295,7 +298,7 @@ int ffai_prefix_attn_fwd(const ffai_kv_cache* prefix, const ffai_kv_cache* own, 
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (pl.block_slots > 0) {
     p.block_slots = pl.block_slots;
-    if (parts == kPartsBoth && p.R <= 16) {  // (an f32 q's parts leave registers for 16 rows)
+    if (parts != kPartsOne && p.R <= 16) {  // (the parts leave registers for 16 rows)
       p.block_slots = std::min(p.per, 16 / p.R);
       p.pre.row_blocks = (p.per + p.block_slots - 1) / p.block_slots;
     }

@@ -33,10 +33,10 @@
 namespace ffai {
 namespace {
 
-// LDS elements of a wave in prefix_work: a V tile and 2 KB, and no less than the merge area
-// (32 rows of D + 4 floats, then their maxima and sums).
+// LDS elements of a wave: its V tiles (two at head_dim 64, see PrefixWave::AHEAD) and 2 KB, and no
+// less than the merge area (32 rows of D + 4 floats, then their maxima and sums).
 template <int D>
-constexpr int kWaveLds = BN * D + 1024;
+constexpr int kWaveLds = (D == 64 ? 2 : 1) * BN * D + 1024;
 
 // What one workgroup attends: its keys and its rows.
 struct PrefixWork {
@@ -67,9 +67,16 @@ struct PrefixWave {
   static constexpr int KC = D / 32;   // contraction chunks of S^T
   static constexpr int OROW = D + 4;  // merge area: rows of O, then maxima, then sums
   static_assert((32 * OROW + 64) * 4 <= kWaveLds<D> * 2, "the merge area fits in the wave's area");
-  static_assert(BN * D * 2 + 32 * 16 * 4 <= kWaveLds<D> * 2, "a V tile and 32 keys' weights fit");
+  // The next tile is loaded under the current one, K into the registers that the scores have read, V
+  // into a second buffer, where registers and LDS have room for it: at head_dim 64 with 16 rows. (At
+  // 128 the buffer would leave room for one workgroup on a CU; two without it stream keys at 5.4 TB/s.)
+  static constexpr bool AHEAD = D == 64 && NC == 1;
+  static constexpr int VBUF = AHEAD ? BN * D : 0;  // from one V buffer to the other
+  static_assert((VBUF + BN * D) * 2 + 32 * 16 * 4 <= kWaveLds<D> * 2, "V tiles and 32 keys' weights");
 
-  uint16_t* vl;  // the wave's LDS
+  uint16_t* base;  // the wave's LDS
+  int cur;         // the V buffer of the tile issued last, elements from base
+  bool careful;    // look for non-finite V before a product that rows share (always where !AHEAD)
   int lane, q4, n16;
   u32x4 qf[NQ][NC][KC];
   float sl2[NC];  // scores to log2 units
@@ -85,7 +92,12 @@ struct PrefixWave {
     lane = item_id() & 63;
     q4 = lane >> 4;
     n16 = lane & 15;
-    vl = lds;
+    base = lds;
+    cur = 0;
+    careful = !AHEAD;
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
 #pragma unroll
@@ -104,7 +116,8 @@ struct PrefixWave {
     const int lr = lane / CH, lc = lane % CH;
     const char* kb = reinterpret_cast<const char*>(k);
     const char* vb = reinterpret_cast<const char*>(v);
-    const uint32_t va = lds_addr(vl);
+    cur ^= VBUF;
+    const uint32_t va = lds_addr(base + cur);
 #pragma unroll
     for (int kb4 = 0; kb4 < 4; ++kb4) {
       const char* kr = kb + 2 * ((uint32_t)min(16 * kb4 + n16, valid - 1) * (uint32_t)s_pos + 8 * q4);
@@ -168,10 +181,13 @@ struct PrefixWave {
   }
 
   // The tile that was issued last, `valid` of its keys there; column block c's row sees its keys up to
-  // lim[c] (all of the valid ones where `cut` is false).
-  __device__ __forceinline__ void tile(int valid, bool cut, const int (&lim)[NC]) {
+  // lim[c] (all of the valid ones where `cut` is false). next() issues the tile after it: under this
+  // one, or once its V is done with.
+  template <class F>
+  __device__ __forceinline__ void tile(int valid, bool cut, const int (&lim)[NC], F next) {
     vm_wait_all();
     asm volatile("" ::: "memory");
+    uint16_t* vl = base + cur;
     if (valid < BN) {
       // V rows past the last key: a masked weight is 0, but 0 times what lies there need not be
       for (int u = valid * CH + lane; u < BN * CH; u += 64)
@@ -180,7 +196,7 @@ struct PrefixWave {
     // Keys that only some of the rows see may hold a non-finite V, which a weight of 0 would let into
     // the other rows: such a tile takes the slow second product.
     bool slow = false;
-    if (cut) {
+    if (cut && careful) {
       bool bad = false;
 #pragma unroll 2
       for (int u = lane; u < BN * CH; u += 64) {
@@ -203,6 +219,10 @@ struct PrefixWave {
 #pragma unroll
           for (int q = NQ - 1; q >= 0; --q)
             s[c][kb4] = mfma16x16<DT>(kf[kb4][h], qf[q][c][h], s[c][kb4]);
+    }
+    if constexpr (AHEAD) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the other buffer's reads are done
+      next();
     }
     if (cut || valid < BN) {
 #pragma unroll
@@ -259,8 +279,8 @@ struct PrefixWave {
 #pragma unroll
         for (int db = 0; db < D / 16; ++db) {
           const int r = 32 * ch + 4 * q4 + tr_row, col = 16 * db + tr_col;
-          const uint16_t* base = &vl[r * D + 8 * swz_v(r, col >> 3) + (col & 7)];
-          const u32x2 a0 = lds_tr(base), a1 = lds_tr(base + 16 * D);
+          const uint16_t* at = &vl[r * D + 8 * swz_v(r, col >> 3) + (col & 7)];
+          const u32x2 a0 = lds_tr(at), a1 = lds_tr(at + 16 * D);
           const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
 #pragma unroll
           for (int c = 0; c < NC; ++c)
@@ -270,7 +290,7 @@ struct PrefixWave {
     } else {
       // key by key, only where the row sees it (the weights through LDS, 32 keys of 16 columns at a
       // time)
-      float* pl = reinterpret_cast<float*>(vl + BN * D);
+      float* pl = reinterpret_cast<float*>(base + VBUF + BN * D);
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -303,6 +323,25 @@ struct PrefixWave {
           asm volatile("" ::: "memory");
         }
     }
+    if constexpr (!AHEAD) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this tile's V reads are done
+      next();
+    }
+  }
+
+  // Whether every result so far is finite (AHEAD: its registers allow a second go). (A row that shares a tile with a non-finite V that it does
+  // not see is not: then the wave starts again, carefully. Results that are rightly non-finite come
+  // out the same from the second go.)
+  __device__ __forceinline__ bool finite() const {
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          bad = bad || (__float_as_uint(oacc[c][db][r]) & 0x7f800000u) == 0x7f800000u;
+    return __ballot(bad) == 0;
   }
 
   // The wave's result to its merge area (after a barrier: tiles are done with).
@@ -383,17 +422,22 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const PrefixW
     x.load_q(p, c, row_offset(p, p.q_ss, p.q_sh, p.q_st, w.slot0 + ds, w.h, rr));
   }
 #pragma unroll 1
-  for (int it = w.t_begin + wave; it < w.t_end; it += NWD) {
-    const int kb = it * BN;
-    if (it != w.t_begin + wave) {
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the area's earlier reads are done
-      issue(it);
-    }
-    int lim[NC];
+  for (;;) {
+#pragma unroll 1
+    for (int it = w.t_begin + wave; it < w.t_end; it += NWD) {
+      const int kb = it * BN;
+      int lim[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) lim[c] = see[c] - kb;
-    // (one query token sees every key of the sequence)
-    x.tile(min(BN, w.n_keys - kb), p.T > 1 && kb + BN - 1 > w.causal_last, lim);
+      for (int c = 0; c < NC; ++c) lim[c] = see[c] - kb;
+      // (one query token sees every key of the sequence)
+      x.tile(min(BN, w.n_keys - kb), p.T > 1 && kb + BN - 1 > w.causal_last, lim, [&] {
+        if (it + NWD < w.t_end) issue(it + NWD);
+      });
+    }
+    if (!Wave::AHEAD || p.T == 1 || x.careful || x.finite()) break;
+    x.clear();
+    x.careful = true;
+    if (w.t_begin + wave < w.t_end) issue(w.t_begin + wave);
   }
   // ---- the waves' results meet in LDS (each wave's area is free once all pass here)
   __syncthreads();
@@ -418,7 +462,7 @@ __device__ __forceinline__ void prefix_work(const PrefixParams& p, const PrefixW
 // Short sequences, one launch and no partials: a workgroup takes a few slots of a group (their rows
 // are the columns, whole slots only) with everything they see of one K/V head: the prefix's tiles,
 // then each slot's own, dealt to the eight waves in turn. A slot's own tile is masked for the other
-// slots' columns; its V is looked over for non-finite values, which must not reach them. Bound by
+// slots' columns. Bound by
 // the chain of a few tiles a wave (~2 us each) and the join.
 template <int DT, int D, int NQ, int NP, int NC, int OUTT>
 __global__ __launch_bounds__(kWholeWaves * 64, 2) void prefix_whole_kernel(PrefixParams p) {
@@ -481,17 +525,22 @@ __global__ __launch_bounds__(kWholeWaves * 64, 2) void prefix_whole_kernel(Prefi
     x.load_q(p, c, row_offset(p, p.q_ss, p.q_sh, p.q_st, slot0 + my_slot[c], h, rr));
   }
 #pragma unroll 1
-  for (int it = wave; it < tiles; it += NWD) {
-    if (it != wave) {
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the area's earlier reads are done
-      issue(it);
-    }
-    int lim[NC];
+  for (;;) {
+#pragma unroll 1
+    for (int it = wave; it < tiles; it += NWD) {
+      int lim[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-      lim[c] = my_slot[c] == t_slot ? t_len - p.T + my_t[c] - t_kb : -1;
-    const bool cut = t_slot >= 0 && (slots > 1 || (p.T > 1 && t_kb + BN - 1 > t_len - p.T));
-    x.tile(min(BN, t_len - t_kb), cut, lim);
+      for (int c = 0; c < NC; ++c)
+        lim[c] = my_slot[c] == t_slot ? t_len - p.T + my_t[c] - t_kb : -1;
+      const bool cut = t_slot >= 0 && (slots > 1 || (p.T > 1 && t_kb + BN - 1 > t_len - p.T));
+      x.tile(min(BN, t_len - t_kb), cut, lim, [&] {
+        if (it + NWD < tiles) issue(it + NWD);
+      });
+    }
+    if (!Wave::AHEAD || x.careful || x.finite()) break;
+    x.clear();
+    x.careful = true;
+    if (wave < tiles) issue(wave);
   }
   __syncthreads();
   float* mbase = reinterpret_cast<float*>(whole_lds);
@@ -719,8 +768,8 @@ __device__ __forceinline__ void prefix_rows(const PrefixParams& p, const PrefixW
 }
 
 // ROWS: the prefix's pieces run as prefix_rows (many rows), else as prefix_work in blocks of 16 NCP
-// rows; the own pieces always as prefix_work. In the first case the two kinds alternate in the grid,
-// so that a CU holds one of each: the prefix's are bound by the matrix cores, the own ones by memory.
+// rows; the own pieces always as prefix_work. The prefix's come first in the grid: 128 slots x 32
+// heads, 16384 shared and 33 to 1024 own keys 107 us, with the two kinds in turn 109 to 119.
 template <int DT, int D, int NQ, int NP, int NCP, int NCO, bool ROWS>
 __global__ __launch_bounds__(kPrefixWaves * 64, NQ > 1 && (NCP > 1 || NCO > 1 || D == 128) ? 1 : 2) void
 prefix_unit_kernel(PrefixParams p) {
@@ -728,15 +777,8 @@ prefix_unit_kernel(PrefixParams p) {
   static_assert(!ROWS || LDS >= 4 * BN * D, "two tiles of K and V fit");
   __shared__ __attribute__((aligned(16))) uint16_t lds[LDS];
   int item = wg_id_x();
-  bool pre;
-  if (ROWS && p.stride > 1) {  // a prefix item, then stride - 1 own ones
-    const int mixed = p.pre.items * p.stride;
-    pre = item < mixed && item % p.stride == 0;
-    item = pre ? item / p.stride : item < mixed ? item - item / p.stride - 1 : item - p.pre.items;
-  } else {
-    pre = item < p.pre.items;
-    if (!pre) item -= p.pre.items;
-  }
+  const bool pre = item < p.pre.items;
+  if (!pre) item -= p.pre.items;
   const PrefixSide& sd = pre ? p.pre : p.own;
   PrefixWork w;
   const int piece = item % sd.pieces;

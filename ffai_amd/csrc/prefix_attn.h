@@ -33,7 +33,6 @@ struct PrefixParams {
   int32_t M;  // rows of a group that read one prefix K/V head: per * R
   int32_t block_slots;  // prefix_whole_kernel: slots of a workgroup
   int32_t many;    // the prefix's pieces in blocks of kPrefixManyRows rows (prefix_rows)
-  int32_t stride;  // then: every stride-th item of the grid's first ones is a prefix piece
   float scale_log2;
 };
 

@@ -85,15 +85,20 @@ class PrefixAttention:
                 out = torch.empty(self.shape, dtype=self.out_dtype, device=self.device)
             elif out.shape != self.shape or out.dtype != self.out_dtype or out.device != self.device:
                 raise ValueError(f"out must be {self.shape} {self.out_dtype} on {self.device}")
+            work, n = None, 0
             if workspace is None:
-                workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
-            elif workspace.device != self.device or not workspace.is_contiguous():
+                if self.workspace_bytes:
+                    workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8,
+                                            device=self.device)
+                    work, n = workspace.data_ptr(), self.workspace_bytes
+            elif workspace.device == self.device and workspace.is_contiguous():
+                work, n = workspace.data_ptr(), workspace.nbytes
+            else:
                 raise ValueError(f"workspace must be contiguous, on {self.device}")
             L.check(L.load().ffai_prefix_attn_fwd(
                 *self._refs, q.data_ptr(), _DT[self.q_dtype], self.heads_q, self.q_len,
                 self._stride_array(q), self.scale, out.data_ptr(), _DT[self.out_dtype],
-                self._stride_array(out), workspace.data_ptr(), workspace.nbytes,
-                L.current_stream(self.device)))
+                self._stride_array(out), work, n, L.current_stream(self.device)))
         return out
 
     __call__ = forward

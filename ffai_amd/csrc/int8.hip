@@ -314,6 +314,118 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
     }
 }
 
+// ---- few rows --------------------------------------------------------------------------------
+// At most 16 rows, quantization and product in one launch: a workgroup takes 16 outputs, quantizes
+// all the rows itself into LDS (they are a few KB, from L2) under its weights' loads, and its eight
+// waves share out the contraction, 64 bytes a step in turn, on v_mfma_i32_16x16x64_i8 (A: the
+// weights' rows, B: the rows of x; lane l: row l % 16, 16 bytes at 16 (l / 16)). LDS rows are padded
+// by 16 bytes, so that the 16 rows of a fragment read cover all banks. The waves' partial sums are
+// integers: their order does not matter. Bound by the launch and the chain of two round trips; a
+// second launch for the quantization alone costs more than doing it in every workgroup.
+constexpr int kFewRows = 16;
+constexpr int kFewWaves = 8;
+constexpr int kFewAhead = 4;            // steps of weights loaded before the rows are quantized
+constexpr int kFewLds = 64 * 1024;      // quantized rows at most
+constexpr int64_t few_lds(int rows, int in_dim) {
+  return (int64_t)rows * ((in_dim + kStep - 1) / kStep * kStep + 16);
+}
+
+template <int DT, int OUT>
+__global__ __launch_bounds__(kFewWaves * 64) void int8_few_kernel(Int8Params p, const void* xv,
+                                                                  int64_t xs, int dim) {
+  extern __shared__ __attribute__((aligned(16))) int8_t few_x[];
+  __shared__ float scales[kFewRows];
+  __shared__ int part[kFewWaves][256];
+  const int tid = item_id(), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int o0 = wg_id_x() * 16, r16 = lane & 15, q4 = lane >> 4;
+  const int8_t* wr = p.w + (int64_t)min(o0 + r16, p.out_dim - 1) * p.ws;
+  const int steps = 2 * p.steps;  // of 64 bytes
+  const int pitch = p.steps * kStep + 16;
+  auto load_w = [&](int s) {
+    return *reinterpret_cast<const i32x4*>(wr + min(64 * s + 16 * q4, p.w_last));
+  };
+  i32x4 a[kFewAhead];
+#pragma unroll
+  for (int j = 0; j < kFewAhead; ++j) a[j] = load_w(wave + kFewWaves * j);
+  // ---- a wave per row: its largest magnitude, then its quotients (from the caches, or registers)
+  for (int m = wave; m < p.rows; m += kFewWaves) {
+    const store_t<DT>* x = reinterpret_cast<const store_t<DT>*>(xv) + (int64_t)m * xs;
+    const int end = p.steps * kStep;
+    int8_t* q = few_x + m * pitch;
+    float v[2][8];
+    uint32_t top = 0;
+#pragma unroll 1
+    for (int k = 8 * lane; k < end; k += 1024) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load8<DT>(x, k + 512 * h, dim, v[h]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, mag(v[h][e]));
+      }
+    }
+    top = wave_umax(top);
+    const float s = row_scale(top);
+    if (lane == 0) scales[m] = s;
+#pragma unroll 1
+    for (int k = 8 * lane; k < end; k += 1024) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (end > 1024) load8<DT>(x, k + 512 * h, dim, v[h]);
+        if (k + 512 * h < end) *reinterpret_cast<u32x2*>(q + k + 512 * h) = quant8(v[h], s);
+      }
+    }
+  }
+  __syncthreads();
+  i32x4 acc = {0, 0, 0, 0};
+  const int8_t* xl = few_x + min(r16, p.rows - 1) * pitch + 16 * q4;
+#pragma unroll
+  for (int j = 0; j < kFewAhead; ++j) {
+    const int s = wave + kFewWaves * j;
+    if (s < steps)  // uniform
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], *reinterpret_cast<const i32x4*>(xl + 64 * s),
+                                                  acc, 0, 0, 0);
+  }
+#pragma unroll 4
+  for (int s = wave + kFewWaves * kFewAhead; s < steps; s += kFewWaves)
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_w(s), *reinterpret_cast<const i32x4*>(xl + 64 * s),
+                                                acc, 0, 0, 0);
+  // D lane l: outputs 4 (l / 16) .. +3 of row l % 16
+  *reinterpret_cast<i32x4*>(&part[wave][4 * lane]) = acc;
+  __syncthreads();
+  if (tid < 256) {
+    const int m = tid >> 4, o = tid & 15;  // rows outermost: 16 outputs of a row in a row
+    if (m < p.rows && o0 + o < p.out_dim) {
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w) sum += part[w][4 * (16 * (o >> 2) + m) + (o & 3)];
+      const float t = (float)sum * scales[m];
+      const float v = p.bias ? __builtin_fmaf(t, p.sw[o0 + o], p.bias[o0 + o]) : t * p.sw[o0 + o];
+      store_t<OUT>* y = reinterpret_cast<store_t<OUT>*>(p.y) + (int64_t)m * p.ys + o0 + o;
+      if constexpr (OUT == kF32) *y = v;
+      else *y = from_f32<OUT>(v);
+    }
+  }
+}
+
+template <int DT, int OUT>
+hipError_t launch_few(const Int8Params& p, const void* x, int64_t xs, int dim, hipStream_t st) {
+  auto kernel = int8_few_kernel<DT, OUT>;
+  static const hipError_t once = hipFuncSetAttribute(
+      reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
+  if (once != hipSuccess) return once;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.out_dim + 15) / 16)), dim3(kFewWaves * 64),
+                     (size_t)few_lds(p.rows, dim), st, p, x, xs, dim);
+  return hipGetLastError();
+}
+template <int DT>
+hipError_t launch_few_out(const Int8Params& p, int32_t y_dtype, const void* x, int64_t xs, int dim,
+                          hipStream_t st) {
+  return y_dtype == FFAI_F32   ? launch_few<DT, kF32>(p, x, xs, dim, st)
+         : y_dtype == FFAI_F16 ? launch_few<DT, kF16>(p, x, xs, dim, st)
+                               : launch_few<DT, kBF16>(p, x, xs, dim, st);
+}
+
 struct Int8Tile {
   int bx, bw, waves, stages;
 };
@@ -391,17 +503,23 @@ hipError_t quantize(const void* x, int32_t dt, int32_t rows, int32_t dim, int64_
   return hipGetLastError();
 }
 
-hipError_t product(const int8_t* q, int64_t qs, const float* sx, int32_t rows, int32_t in_dim,
-                   const int8_t* w, int64_t ws, const float* sw, const float* bias,
-                   int32_t out_dim, void* y, int32_t y_dtype, int64_t ys, hipStream_t st) {
+Int8Params product_params(const int8_t* q, int64_t qs, const float* sx, int32_t rows,
+                          int32_t in_dim, const int8_t* w, int64_t ws, const float* sw,
+                          const float* bias, int32_t out_dim, void* y, int64_t ys) {
   Int8Params p{};
   p.x = q; p.xs = qs; p.sx = sx; p.w = w; p.ws = ws; p.sw = sw; p.bias = bias;
   p.y = y; p.ys = ys; p.rows = rows; p.out_dim = out_dim;
   p.steps = (in_dim + kStep - 1) / kStep;
   p.w_last = (in_dim + 15) / 16 * 16 - 16;
+  return p;
+}
+hipError_t product(const Int8Params& p, int32_t y_dtype, hipStream_t st) {
   return y_dtype == FFAI_F32   ? launch_product<kF32>(p, st)
          : y_dtype == FFAI_F16 ? launch_product<kF16>(p, st)
                                : launch_product<kBF16>(p, st);
+}
+bool few(int32_t rows, int32_t in_dim) {
+  return rows <= kFewRows && few_lds(rows, in_dim) <= kFewLds;
 }
 
 int64_t row_bytes(int32_t dim) { return ((int64_t)dim + kStep - 1) / kStep * kStep; }
@@ -448,8 +566,9 @@ int ffai_int8_product(const int8_t* q, int64_t q_row_stride, const float* scale,
   if ((uintptr_t)scale % 4) return api_fail(FFAI_ERR_INVALID, "scale must be 4-byte aligned");
   rc = api_check_device();
   if (rc != FFAI_OK) return rc;
-  const hipError_t e = product(q, q_row_stride, scale, rows, in_dim, w, w_row_stride, w_scale, bias,
-                               out_dim, y, y_dtype, y_row_stride, static_cast<hipStream_t>(stream));
+  const hipError_t e = product(product_params(q, q_row_stride, scale, rows, in_dim, w, w_row_stride,
+                                              w_scale, bias, out_dim, y, y_row_stride),
+                               y_dtype, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));
   return FFAI_OK;
 }
@@ -459,7 +578,8 @@ int ffai_int8_linear_workspace_bytes(int32_t rows, int32_t in_dim, size_t* bytes
   if (!bytes) return api_fail(FFAI_ERR_INVALID, "null bytes pointer");
   const int rc = check_dims(rows, in_dim);
   if (rc != FFAI_OK) return rc;
-  *bytes = (size_t)rows * row_bytes(in_dim) + (((size_t)rows * 4 + 15) & ~size_t(15));
+  *bytes = few(rows, in_dim)
+               ? 0 : (size_t)rows * row_bytes(in_dim) + (((size_t)rows * 4 + 15) & ~size_t(15));
   return FFAI_OK;
 }
 
@@ -475,7 +595,7 @@ int ffai_int8_linear(const void* x, int32_t x_dtype, int64_t x_row_stride, int32
   if (rows == 0) return FFAI_OK;
   size_t need = 0;
   ffai_int8_linear_workspace_bytes(rows, in_dim, &need);
-  if (!workspace || workspace_bytes < need)
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return api_fail(FFAI_ERR_WORKSPACE, "workspace smaller than ffai_int8_linear_workspace_bytes");
   if ((uintptr_t)workspace % 16) return api_fail(FFAI_ERR_INVALID, "workspace must be 16-byte aligned");
   rc = api_check_device();
@@ -483,10 +603,17 @@ int ffai_int8_linear(const void* x, int32_t x_dtype, int64_t x_row_stride, int32
   hipStream_t st = static_cast<hipStream_t>(stream);
   int8_t* q = static_cast<int8_t*>(workspace);
   float* sx = reinterpret_cast<float*>(q + (size_t)rows * row_bytes(in_dim));
-  hipError_t e = quantize(x, x_dtype, rows, in_dim, x_row_stride, q, row_bytes(in_dim), sx, st);
-  if (e == hipSuccess)
-    e = product(q, row_bytes(in_dim), sx, rows, in_dim, w, w_row_stride, w_scale, bias, out_dim, y,
-                y_dtype, y_row_stride, st);
+  const Int8Params p = product_params(q, row_bytes(in_dim), sx, rows, in_dim, w, w_row_stride, w_scale,
+                                      bias, out_dim, y, y_row_stride);
+  hipError_t e;
+  if (few(rows, in_dim)) {
+    e = x_dtype == FFAI_F32   ? launch_few_out<kF32>(p, y_dtype, x, x_row_stride, in_dim, st)
+        : x_dtype == FFAI_F16 ? launch_few_out<kF16>(p, y_dtype, x, x_row_stride, in_dim, st)
+                              : launch_few_out<kBF16>(p, y_dtype, x, x_row_stride, in_dim, st);
+  } else {
+    e = quantize(x, x_dtype, rows, in_dim, x_row_stride, q, row_bytes(in_dim), sx, st);
+    if (e == hipSuccess) e = product(p, y_dtype, st);
+  }
   if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));
   return FFAI_OK;
 }

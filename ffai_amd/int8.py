@@ -128,14 +128,18 @@ class Int8Linear:
         with L.on_device(device):
             out, yp, ys = self._out((*x.shape[:-1], self.out_dim), rows, dtype, out, device)
             if workspace is None:
-                # ffai_int8_linear_workspace_bytes: the padded rows, then their scales
-                n = rows * (-(-self.in_dim // _PAD) * _PAD) + (rows * 4 + 15) // 16 * 16
-                workspace = torch.empty(n, dtype=torch.uint8, device=device)
-            elif workspace.device != device or not workspace.is_contiguous():
+                n = self.workspace_bytes(rows)
+                work = None
+                if n:
+                    workspace = torch.empty(n, dtype=torch.uint8, device=device)
+                    work = workspace.data_ptr()
+            elif workspace.device == device and workspace.is_contiguous():
+                work, n = workspace.data_ptr(), workspace.nbytes
+            else:
                 raise ValueError(f"workspace must be contiguous, on {device}")
             L.check(L.load().ffai_int8_linear(
                 x2.data_ptr(), _DT[x2.dtype], x2.stride(0), rows, self.in_dim, *self._w, yp,
-                _DT[dtype], ys, workspace.data_ptr(), workspace.nbytes, L.current_stream(device)))
+                _DT[dtype], ys, work, n, L.current_stream(device)))
         return out
 
     __call__ = forward

@@ -52,7 +52,8 @@ int ffai_int8_product(const int8_t* q, int64_t q_row_stride, const float* scale,
                       int64_t y_row_stride, void* stream);
 
 /* Both of them: y from x. The workspace holds the quantized rows for the time of the call: it
- * needs no clearing; calls that may overlap need one each. 16-byte aligned. */
+ * needs no clearing; calls that may overlap need one each. 16-byte aligned. Few rows need none (0
+ * bytes; then it may be NULL). */
 int ffai_int8_linear(const void* x, int32_t x_dtype, int64_t x_row_stride, int32_t rows,
                      int32_t in_dim, const int8_t* w, int64_t w_row_stride, const float* w_scale,
                      const float* bias, int32_t out_dim, void* y, int32_t y_dtype,

@@ -88,6 +88,7 @@ def test_halves_small_and_non_finite_rows(gpu):
 
 
 SIZES = [(1, 1, 1), (1, 128, 32), (2, 100, 31), (5, 1024, 1024), (16, 640, 48), (17, 130, 65),
+         (1, 2081, 100), (16, 4000, 33), (16, 4100, 40), (3, 9001, 17), (1, 65408, 20), (2, 40000, 20),
          (33, 257, 70), (64, 128, 64), (65, 129, 63), (100, 1000, 130), (130, 64, 700),
          (300, 2100, 129), (257, 512, 257)]
 
@@ -216,8 +217,8 @@ def test_streams_and_graph_replays(gpu):
 
 def test_short_workspace_is_refused(gpu):
     lin, *_ = layer(gpu, 40, 96, False)
-    x = rand(gpu, 6, 96)
-    n = lin.workspace_bytes(6)
+    x = rand(gpu, 22, 96)
+    n = lin.workspace_bytes(22)
     lin(x, workspace=torch.empty(n, dtype=torch.uint8, device=gpu))
     with pytest.raises(L.FfaiError, match="workspace"):
         lin(x, workspace=torch.empty(n - 1, dtype=torch.uint8, device=gpu))

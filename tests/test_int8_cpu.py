@@ -85,12 +85,17 @@ def test_no_rows_is_no_work():
 
 
 def test_workspace():
-    rc, msg = linear(work=0)
+    rc, msg = linear(rows=20, work=0)
     assert rc == L.FFAI_ERR_WORKSPACE and "workspace" in msg
     n = ctypes.c_size_t()
-    assert L.load().ffai_int8_linear_workspace_bytes(5, 129, ctypes.byref(n)) == L.FFAI_OK
-    assert n.value == 5 * 256 + 32
-    assert linear(rows=5, dim=129, xs=129, work_bytes=n.value - 1)[0] == L.FFAI_ERR_WORKSPACE
+    assert L.load().ffai_int8_linear_workspace_bytes(50, 129, ctypes.byref(n)) == L.FFAI_OK
+    assert n.value == 50 * 256 + 208
+    assert linear(rows=50, dim=129, xs=129, work_bytes=n.value - 1)[0] == L.FFAI_ERR_WORKSPACE
+    # few rows are quantized where they are used, unless they are too long for that
+    for rows, dim, none in ((1, 1, True), (16, 1024, True), (17, 1024, False), (16, 4080, False),
+                            (1, 65408, True), (1, 65536, False)):
+        assert L.load().ffai_int8_linear_workspace_bytes(rows, dim, ctypes.byref(n)) == L.FFAI_OK
+        assert (n.value == 0) == none, (rows, dim, n.value)
 
 
 def test_binding_refuses():

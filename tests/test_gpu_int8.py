@@ -87,6 +87,28 @@ def test_halves_small_and_non_finite_rows(gpu):
     same(lin(x.to(gpu)), oracle8.linear(q, s, w, sw), False)
 
 
+@pytest.mark.parametrize("rows,dim", [(9, 5000), (1030, 4096), (3, 16384)])
+def test_quotients_next_to_a_half(gpu, rows, dim):
+    """Rows whose quotients lie on halves, some units in the last place off them, and 1e-5 to 1e-4
+    off: which integer each goes to is the division's."""
+    g = np.random.default_rng(dim)
+    top = np.float32(1) + g.random((rows, 1), dtype=np.float32)
+    s = top / np.float32(127)
+    half = g.integers(-127, 127, (rows, dim)).astype(np.float32) + np.float32(0.5)
+    x = (half * s).astype(np.float32)
+    ulps = g.integers(-3, 4, (rows, dim)).astype(np.int32)
+    x = (x.view(np.int32) + ulps).view(np.float32)
+    x[:, 1::3] += (g.uniform(-1e-4, 1e-4, (rows, dim)).astype(np.float32) * s)[:, 1::3]
+    x[:, :1] = top
+    qr = quantize_rows(torch.from_numpy(x).to(gpu))
+    q, scale = oracle8.quantize_rows(x)
+    assert np.array_equal(qr.scale.cpu().numpy(), scale)
+    assert np.array_equal(qr.q[:, :dim].cpu().numpy(), q)
+    lin, w, sw, b = layer(gpu, 33, dim, False)
+    for m in (1, 3, rows):  # and where they are quantized inside the product
+        same(lin(torch.from_numpy(x[:m]).to(gpu)), oracle8.linear(q[:m], scale[:m], w, sw), False)
+
+
 SIZES = [(1, 1, 1), (1, 128, 32), (2, 100, 31), (5, 1024, 1024), (16, 640, 48), (17, 130, 65),
          (1, 2081, 100), (16, 4000, 33), (16, 4100, 40), (3, 9001, 17), (1, 65408, 20), (2, 40000, 20),
          (33, 257, 70), (64, 128, 64), (65, 129, 63), (100, 1000, 130), (130, 64, 700),

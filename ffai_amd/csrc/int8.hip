@@ -267,7 +267,8 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
   const char* xb = reinterpret_cast<const char*>(p.x + (int64_t)x0 * p.xs);
   const char* wb = reinterpret_cast<const char*>(p.w + (int64_t)w0 * p.ws);
   const int lr = lane >> 3;
-  const int chunk = 16 * ((lane & 7) ^ lr);
+  const int chunk[2] = {16 * ((lane & 7) ^ (lr >> 1)), 16 * ((lane & 7) ^ (4 + (lr >> 1)))};
+  static_assert(PB % 2 == 0 && BW % 16 == 0, "a wave's blocks begin at even ones");
   uint32_t off[PB];
 #pragma unroll
   for (int b = 0; b < PB; ++b) {
@@ -277,12 +278,16 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
   }
   const uint32_t lds0 = lds_addr(int8_lds) + wave * PB * 1024;
   auto issue = [&](int step, int buf) {
-    const uint32_t kx = (uint32_t)(step * kStep + chunk);
-    const uint32_t kw = min(kx, (uint32_t)p.w_last);
+    uint32_t kx[2], kw[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      kx[b] = (uint32_t)(step * kStep + chunk[b]);
+      kw[b] = min(kx[b], (uint32_t)p.w_last);
+    }
 #pragma unroll
     for (int b = 0; b < PB; ++b) {
       const bool of_w = (wave * PB + b) * 8 < BW;  // wave-uniform
-      lds_dma16_sbase(of_w ? wb : xb, off[b] + (of_w ? kw : kx), lds0 + buf * BUF + b * 1024);
+      lds_dma16_sbase(of_w ? wb : xb, off[b] + (of_w ? kw[b & 1] : kx[b & 1]), lds0 + buf * BUF + b * 1024);
     }
   };
 
@@ -295,35 +300,47 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
+  for (int s = 0; s < STAGES; ++s)
     if (s < p.steps) issue(s, s);
   const int row = lane & 31, half = lane >> 5;
-  int buf = 0, nbuf = STAGES - 1;
-#pragma unroll 1
-  for (int step = 0; step < p.steps; ++step) {
+  constexpr int KS = kStep / 32;
+  i32x4 a[2][FW], b[2][FX];
+  auto frags = [&](int buf, int ks, i32x4 (&fa)[FW], i32x4 (&fb)[FX]) {
+    const int8_t* base = int8_lds + buf * BUF;
+    const int8_t* wl = base + (gw * FW * 32 + row) * kStep;
+    const int8_t* xl = base + (BW + gx * FX * 32 + row) * kStep;
+    const int c = 16 * ((2 * ks + half) ^ ((row >> 1) & 7));
+#pragma unroll
+    for (int i = 0; i < FW; ++i) fa[i] = *reinterpret_cast<const i32x4*>(wl + i * 32 * kStep + c);
+#pragma unroll
+    for (int j = 0; j < FX; ++j) fb[j] = *reinterpret_cast<const i32x4*>(xl + j * 32 * kStep + c);
+  };
+  // the loads of `step` of every wave have landed, and every wave's reads so far are done
+  auto meet = [&](int step) {
     asm volatile("" ::: "memory");
     if (STAGES > 2 && step + STAGES - 2 < p.steps) wait_vm<PB*(STAGES - 2)>();
     else wait_vm<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (step + STAGES - 1 < p.steps) issue(step + STAGES - 1, nbuf);
-    const int8_t* base = int8_lds + buf * BUF;
-    const int8_t* wl = base + (gw * FW * 32 + row) * kStep;
-    const int8_t* xl = base + (BW + gx * FX * 32 + row) * kStep;
-    // fragments of the next 32 bytes are read under the products of the current ones (the
-    // scheduling barriers keep the compiler from reading all of them first, which spills)
-    i32x4 a[2][FW], b[2][FX];
-    auto frags = [&](int ks, i32x4 (&fa)[FW], i32x4 (&fb)[FX]) {
-      const int c = 16 * ((2 * ks + half) ^ (row & 7));
+  };
+  if (STAGES <= p.steps) wait_vm<PB*(STAGES - 1)>();
+  else wait_vm<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  frags(0, 0, a[0], b[0]);
+  int buf = 0;
+#pragma unroll 1
+  for (int step = 0; step < p.steps; ++step) {
+    const int nbuf = buf + 1 == STAGES ? 0 : buf + 1;
 #pragma unroll
-      for (int i = 0; i < FW; ++i) fa[i] = *reinterpret_cast<const i32x4*>(wl + i * 32 * kStep + c);
-#pragma unroll
-      for (int j = 0; j < FX; ++j) fb[j] = *reinterpret_cast<const i32x4*>(xl + j * 32 * kStep + c);
-    };
-    frags(0, a[0], b[0]);
-#pragma unroll
-    for (int ks = 0; ks < kStep / 32; ++ks) {
-      if (ks + 1 < kStep / 32) frags(ks + 1, a[(ks + 1) & 1], b[(ks + 1) & 1]);
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS) {
+        frags(buf, ks + 1, a[(ks + 1) & 1], b[(ks + 1) & 1]);
+      } else if (step + 1 < p.steps) {
+        meet(step + 1);
+        frags(nbuf, 0, a[0], b[0]);
+        if (step + STAGES < p.steps) issue(step + STAGES, buf);
+      }
 #pragma unroll
       for (int i = 0; i < FW; ++i)
 #pragma unroll
@@ -332,8 +349,7 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
                                                             0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
-    buf = buf + 1 == STAGES ? 0 : buf + 1;
-    nbuf = nbuf + 1 == STAGES ? 0 : nbuf + 1;
+    buf = nbuf;
   }
 
   // ---- D lane l, element 4 q + r: w row 8 q + 4 (l / 32) + r, x row l % 32. Through the wave's
@@ -344,7 +360,7 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
   constexpr int P = FW * 32 * ES;  // bytes of a row of the wave's tile
   constexpr int AREA = BUF * STAGES / NW;
   constexpr int JP = FX < AREA / (32 * P) ? FX : AREA / (32 * P);  // row blocks at a time
-  static_assert(JP >= 1 && FX % JP == 0 && (P == 64 || P == 128 || P == 256), "");
+  static_assert(JP >= 1 && FX % JP == 0 && P >= 64 && P <= 512, "");
   constexpr int LPR = P / 16, RPI = 64 / LPR;  // lanes of a row, rows of a store
   auto key = [](int r) { return P == 64 ? (r >> 1) & 3 : r & 7; };
   int8_t* area = int8_lds + wave * AREA;

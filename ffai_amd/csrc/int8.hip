@@ -236,11 +236,18 @@ __device__ __forceinline__ void wait_vm() {
 // v_mfma_i32_32x32x32_i8 (lane l: row l % 32, 16 bytes at 16 (l / 32) of the 32): the weights are
 // the A operand, so a lane's results are four consecutive outputs of one row of x. Steps of 128
 // bytes of the contraction arrive by DMA in a ring of STAGES buffers, rows unpadded with their eight
-// 16-byte chunks XOR-permuted by the row's low bits, so that the DMA's lanes read whole 128-byte
-// rows and eight lanes of a fragment read cover all banks. One barrier a step: it says that the
-// step's loads of every wave have landed and that every wave has read the buffer the next loads
-// overwrite. Rows past the operands' ends are clamped (their results are not stored); contraction
-// bytes past in_dim are zero in x, so whatever w's clamped chunk holds there counts for nothing.
+// 16-byte chunks XOR-permuted by the row's number / 2, so that the DMA's lanes read whole 128-byte
+// rows and the sixteen lanes of one cycle of a fragment read cover all 64 banks (by the row's low
+// bits instead, rows r and r + 8 collide: half of all LDS cycles). One barrier a step, before its last
+// products: it says that the next step's loads of every wave have landed and that every wave has
+// read this step's buffer, which the loads begun there overwrite; the next step's first fragments
+// are read under those products. Rows past the operands' ends are clamped (their results are not
+// stored); contraction bytes past in_dim are zero in x, so whatever w's clamped chunk holds there
+// counts for nothing.
+//
+// Bound by the matrix cores at the clock that their power leaves: 24000 x 10240 x 1280 takes 295 us
+// (2.1 POPS), 233 of them with the loop's loads left out; 24000 x 5120 x 1280 155 us, 24000 x 1280 x
+// 1280 51 (its 61 MB of results and the tiles' first loads are 20 of them).
 template <int BX, int BW, int GX, int GW, int STAGES, int OCC, int OUT>
 __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8Params p) {
   constexpr int NW = GX * GW;
@@ -277,17 +284,13 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
                     : (uint32_t)min(r - BW, p.rows - 1 - x0) * (uint32_t)p.xs;
   }
   const uint32_t lds0 = lds_addr(int8_lds) + wave * PB * 1024;
-  auto issue = [&](int step, int buf) {
-    uint32_t kx[2], kw[2];
+  auto issue = [&](int step, int buf, int b0, int b1) {  // blocks b0 .. b1 - 1 of the wave's PB
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      kx[b] = (uint32_t)(step * kStep + chunk[b]);
-      kw[b] = min(kx[b], (uint32_t)p.w_last);
-    }
-#pragma unroll
-    for (int b = 0; b < PB; ++b) {
+    for (int b = b0; b < b1; ++b) {
       const bool of_w = (wave * PB + b) * 8 < BW;  // wave-uniform
-      lds_dma16_sbase(of_w ? wb : xb, off[b] + (of_w ? kw[b & 1] : kx[b & 1]), lds0 + buf * BUF + b * 1024);
+      const uint32_t kx = (uint32_t)(step * kStep + chunk[b & 1]);
+      lds_dma16_sbase(of_w ? wb : xb, off[b] + (of_w ? min(kx, (uint32_t)p.w_last) : kx),
+                      lds0 + buf * BUF + b * 1024);
     }
   };
 
@@ -301,7 +304,7 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
 
 #pragma unroll
   for (int s = 0; s < STAGES; ++s)
-    if (s < p.steps) issue(s, s);
+    if (s < p.steps) issue(s, s, 0, PB);
   const int row = lane & 31, half = lane >> 5;
   constexpr int KS = kStep / 32;
   i32x4 a[2][FW], b[2][FX];
@@ -332,6 +335,8 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
 #pragma unroll 1
   for (int step = 0; step < p.steps; ++step) {
     const int nbuf = buf + 1 == STAGES ? 0 : buf + 1;
+    constexpr int NM = FX * FW;
+    const bool more = step + STAGES < p.steps;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if (ks + 1 < KS) {
@@ -339,14 +344,17 @@ __global__ __launch_bounds__((GX * GW) * 64, OCC) void int8_product_kernel(Int8P
       } else if (step + 1 < p.steps) {
         meet(step + 1);
         frags(nbuf, 0, a[0], b[0]);
-        if (step + STAGES < p.steps) issue(step + STAGES, buf);
       }
 #pragma unroll
-      for (int i = 0; i < FW; ++i)
-#pragma unroll
-        for (int j = 0; j < FX; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks & 1][i], b[ks & 1][j], acc[i][j],
-                                                            0, 0, 0);
+      for (int n = 0; n < NM; ++n) {
+        const int i = n / FX, j = n % FX;
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks & 1][i], b[ks & 1][j], acc[i][j],
+                                                          0, 0, 0);
+        if (ks + 1 == KS && more) {
+          issue(step + STAGES, buf, n * PB / NM, (n + 1) * PB / NM);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     buf = nbuf;

@@ -252,38 +252,24 @@ def get_fwd_split_override() -> tuple:
     return a.value, b.value
 
 
-class _Here:
-    """The context of a device that is the current one already."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def on_device(device):
-    """A context in which `device` (of a tensor) is the current one: library calls launch on the
-    current device. Free where it already is. (Operands of host memory: nothing to select; the
-    library refuses or the caller has checked.)"""
+def call_on(device, fn, *args) -> int:
+    """check(fn(*args, stream)) with `device` (of a tensor) the current one, on its current stream:
+    library calls launch on the current device. (No context where it is that already; the raw
+    stream handle, no Stream object around it. Operands of host memory are refused.)"""
     import torch
 
     if device.type != "cuda":
         raise ValueError(f"operands must be on a HIP device, not {device}")
-    if device.index is None or device.index == torch._C._cuda_getDevice():
-        return _HERE
-    return torch.cuda.device(device)
-
-
-def current_stream(device) -> int:
-    """The raw handle of `device`'s current stream (no Stream object around it)."""
-    import torch
-
-    index = torch._C._cuda_getDevice() if device.index is None else device.index
-    return torch._C._cuda_getCurrentRawStream(index)
+    here = torch._C._cuda_getDevice()
+    index = here if device.index is None else device.index
+    if index == here:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc < 0:
+        raise FfaiError(rc, last_error())
+    return rc
 
 
 def last_error() -> str:

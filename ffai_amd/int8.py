@@ -28,13 +28,14 @@ class QuantizedRows(NamedTuple):
 
 def _rows_view(x: torch.Tensor, dim: int) -> torch.Tensor:
     """x (..., dim) as (rows, dim): a view wherever one stride spans the rows."""
-    if x.dim() < 1 or x.shape[-1] != dim:
-        raise ValueError(f"x must be (..., {dim}), not {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] != dim:
+        raise ValueError(f"x must be (..., {dim}), not {tuple(shape)}")
     if x.dtype not in _DT:
         raise ValueError(f"x must be f32, f16 or bf16, not {x.dtype}")
-    if x.dim() != 2:
+    if len(shape) != 2:
         x = x.reshape(-1, dim)
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < dim):
+    if not x.is_contiguous() and (x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < dim)):
         x = x.contiguous()
     return x
 
@@ -45,12 +46,10 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
         raise ValueError("x must be (rows, dim)")
     rows, dim = x.shape
     x = _rows_view(x, dim)
-    with L.on_device(x.device):
-        q = torch.empty(rows, (dim + _PAD - 1) // _PAD * _PAD, dtype=torch.int8, device=x.device)
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-        L.check(L.load().ffai_int8_quantize_rows(
-            x.data_ptr(), _DT[x.dtype], rows, dim, x.stride(0), q.data_ptr(), q.shape[1],
-            scale.data_ptr(), L.current_stream(x.device)))
+    q = torch.empty(rows, (dim + _PAD - 1) // _PAD * _PAD, dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    L.call_on(x.device, L.load().ffai_int8_quantize_rows, x.data_ptr(), _DT[x.dtype], rows, dim,
+              x.stride(0), q.data_ptr(), q.shape[1], scale.data_ptr())
     return QuantizedRows(q, scale, dim)
 
 
@@ -91,6 +90,9 @@ class Int8Linear:
         self.out_dim, self.in_dim = qw.shape[0], in_dim
         self._w = (qw.data_ptr(), qw.stride(0), scale.data_ptr(),
                    None if bias is None else bias.data_ptr(), self.out_dim)
+        self._few = 0  # up to so many rows need no workspace
+        while self._few < 64 and self.workspace_bytes(self._few + 1) == 0:
+            self._few += 1
 
     def workspace_bytes(self, rows: int) -> int:
         n = ctypes.c_size_t(0)
@@ -125,21 +127,18 @@ class Int8Linear:
         dtype = out_dtype or (x.dtype if out is None else out.dtype)
         x2 = _rows_view(x, self.in_dim)
         rows = x2.shape[0]
-        with L.on_device(device):
-            out, yp, ys = self._out((*x.shape[:-1], self.out_dim), rows, dtype, out, device)
-            if workspace is None:
-                n = self.workspace_bytes(rows)
-                work = None
-                if n:
-                    workspace = torch.empty(n, dtype=torch.uint8, device=device)
-                    work = workspace.data_ptr()
-            elif workspace.device == device and workspace.is_contiguous():
-                work, n = workspace.data_ptr(), workspace.nbytes
-            else:
+        out, yp, ys = self._out((*x.shape[:-1], self.out_dim), rows, dtype, out, device)
+        work, n = None, 0
+        if workspace is not None:
+            if workspace.device != device or not workspace.is_contiguous():
                 raise ValueError(f"workspace must be contiguous, on {device}")
-            L.check(L.load().ffai_int8_linear(
-                x2.data_ptr(), _DT[x2.dtype], x2.stride(0), rows, self.in_dim, *self._w, yp,
-                _DT[dtype], ys, work, n, L.current_stream(device)))
+            work, n = workspace.data_ptr(), workspace.nbytes
+        elif rows > self._few:
+            n = self.workspace_bytes(rows)
+            workspace = torch.empty(n, dtype=torch.uint8, device=device)
+            work = workspace.data_ptr()
+        L.call_on(device, L.load().ffai_int8_linear, x2.data_ptr(), _DT[x2.dtype], x2.stride(0), rows,
+                  self.in_dim, *self._w, yp, _DT[dtype], ys, work, n)
         return out
 
     __call__ = forward
@@ -154,11 +153,9 @@ class Int8Linear:
             raise ValueError("x must be as quantize_rows returns it")
         rows = x.q.shape[0]
         dtype = out_dtype or (torch.float32 if out is None else out.dtype)
-        with L.on_device(device):
-            out, yp, ys = self._out((rows, self.out_dim), rows, dtype, out, device)
-            L.check(L.load().ffai_int8_product(
-                x.q.data_ptr(), x.q.stride(0), x.scale.data_ptr(), rows, self.in_dim, *self._w, yp,
-                _DT[dtype], ys, L.current_stream(device)))
+        out, yp, ys = self._out((rows, self.out_dim), rows, dtype, out, device)
+        L.call_on(device, L.load().ffai_int8_product, x.q.data_ptr(), x.q.stride(0),
+                  x.scale.data_ptr(), rows, self.in_dim, *self._w, yp, _DT[dtype], ys)
         return out
 
 

@@ -80,25 +80,22 @@ class PrefixAttention:
         if q.shape != self.shape or q.dtype != self.q_dtype or q.device != self.device:
             raise ValueError(f"q must be {self.shape} {self.q_dtype} on {self.device}, "
                              f"not {tuple(q.shape)} {q.dtype} on {q.device}")
-        with L.on_device(self.device):
-            if out is None:
-                out = torch.empty(self.shape, dtype=self.out_dtype, device=self.device)
-            elif out.shape != self.shape or out.dtype != self.out_dtype or out.device != self.device:
-                raise ValueError(f"out must be {self.shape} {self.out_dtype} on {self.device}")
-            work, n = None, 0
-            if workspace is None:
-                if self.workspace_bytes:
-                    workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8,
-                                            device=self.device)
-                    work, n = workspace.data_ptr(), self.workspace_bytes
-            elif workspace.device == self.device and workspace.is_contiguous():
-                work, n = workspace.data_ptr(), workspace.nbytes
-            else:
+        if out is None:
+            out = torch.empty(self.shape, dtype=self.out_dtype, device=self.device)
+        elif out.shape != self.shape or out.dtype != self.out_dtype or out.device != self.device:
+            raise ValueError(f"out must be {self.shape} {self.out_dtype} on {self.device}")
+        work, n = None, 0
+        if workspace is not None:
+            if workspace.device != self.device or not workspace.is_contiguous():
                 raise ValueError(f"workspace must be contiguous, on {self.device}")
-            L.check(L.load().ffai_prefix_attn_fwd(
-                *self._refs, q.data_ptr(), _DT[self.q_dtype], self.heads_q, self.q_len,
-                self._stride_array(q), self.scale, out.data_ptr(), _DT[self.out_dtype],
-                self._stride_array(out), work, n, L.current_stream(self.device)))
+            work, n = workspace.data_ptr(), workspace.nbytes
+        elif self.workspace_bytes:
+            n = self.workspace_bytes
+            workspace = torch.empty(n, dtype=torch.uint8, device=self.device)
+            work = workspace.data_ptr()
+        L.call_on(self.device, L.load().ffai_prefix_attn_fwd, *self._refs, q.data_ptr(),
+                  _DT[self.q_dtype], self.heads_q, self.q_len, self._stride_array(q), self.scale,
+                  out.data_ptr(), _DT[self.out_dtype], self._stride_array(out), work, n)
         return out
 
     __call__ = forward

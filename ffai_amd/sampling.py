@@ -59,19 +59,20 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = None
     k = _setting(top_k, 0, torch.int32, rows, device, "top_k")
     p = _setting(top_p, 1.0, torch.float32, rows, device, "top_p")
     mp = _setting(min_p, 0.0, torch.float32, rows, device, "min_p")
-    with L.on_device(device):
-        if out is None:
-            out = torch.empty(rows, dtype=torch.int32, device=device)
-        elif out.dtype != torch.int32 or out.shape != (rows,) or out.device != device or \
-                not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous int32 tensor of {rows} on {device}")
-        lp = torch.empty(rows, dtype=torch.float32, device=device) if logprobs else None
-        if workspace is None:
-            workspace = torch.empty(workspace_bytes(rows, vocab), dtype=torch.uint8, device=device)
-        elif workspace.device != device or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be contiguous, on {device}")
-        L.check(L.load().ffai_sample(
-            logits.data_ptr(), _DT[logits.dtype], rows, vocab, logits.stride(0), *t, *k, *p, *mp,
-            u.data_ptr(), out.data_ptr(), None if lp is None else lp.data_ptr(),
-            workspace.data_ptr(), workspace.nbytes, L.current_stream(device)))
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=device)
+    elif out.dtype != torch.int32 or out.shape != (rows,) or out.device != device or \
+            not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous int32 tensor of {rows} on {device}")
+    lp = torch.empty_like(u) if logprobs else None
+    if workspace is None:
+        n = workspace_bytes(rows, vocab)
+        workspace = torch.empty(n, dtype=torch.uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous, on {device}")
+    else:
+        n = workspace.nbytes
+    L.call_on(device, L.load().ffai_sample, logits.data_ptr(), _DT[logits.dtype], rows, vocab,
+              logits.stride(0), *t, *k, *p, *mp, u.data_ptr(), out.data_ptr(),
+              None if lp is None else lp.data_ptr(), workspace.data_ptr(), n)
     return out, lp

@@ -20,6 +20,7 @@
 #include "../../include/ffai_sample.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.cuh"
 
@@ -30,10 +31,13 @@ constexpr int kGroup = 1024;  // elements whose maximum and sums a scan wave lea
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kPick = 1024;   // threads of a pick workgroup
 constexpr int kWaves = kPick / 64;
+constexpr int kSpread = 512;  // threads of a spread workgroup
 constexpr int kShort = 256;   // tokens of a list that one wave finishes
 constexpr int kList = 2048;   // tokens of an LDS list
 constexpr int kBins = 4096;
 constexpr int kChunk = 4096;  // elements of a gather workgroup's share
+constexpr int kParts = 16;    // gather workgroups of a row, about
+constexpr int kCutBins = 2048;  // bins of a nucleus' histogram
 constexpr int kAhead = 4;     // steps of a pass over a row that a wave loads ahead
 
 struct SampleParams {
@@ -56,6 +60,13 @@ struct SampleParams {
   float* low;      // [row] the least logit that is listed; -inf: no list
   int32_t* count;  // [row][chunk] listed tokens (kShort at most are held)
   uint64_t* cand;  // [row][chunk][kShort] their ranks, in no order
+  int32_t per, parts;  // chunks of a gather workgroup, and such workgroups of a row
+  uint32_t* hist;   // [row][part][kCutBins] nuclei: weights by distance from the maximum
+  double* sum_k;    // [row][group] minima: sum of the weights >= min_p
+  double* sum_a;    // [row][group] nuclei: sum of the weights above the boundary's bins
+  int32_t* count2;  // [row][chunk] tokens in the boundary's bins (kShort at most are held)
+  uint64_t* cand2;  // [row][chunk][kShort] their ranks, in no order
+  int32_t* cut;     // [row] nuclei that the list does not settle: whether the boundary's bins are listed
 };
 
 // The device code is compiled for numbers that are not NaN, so NaN is recognised by its bits, and
@@ -312,30 +323,49 @@ __device__ __forceinline__ uint64_t rank_of(float l, int i) {
 __device__ __forceinline__ float logit_of(uint64_t r) { return of_key((uint32_t)(r >> 32)); }
 __device__ __forceinline__ int index_of(uint64_t r) { return (int)(0xffffffffu - (uint32_t)r); }
 
+// LDS of a spread workgroup, and what the block functions below need of one.
+struct SpreadShared {
+  static constexpr int NW = kSpread / 64;
+  uint64_t raw[kShort];  // ranks as collected
+  double red[NW];
+  double sums[2][kChunk / 256];
+  int i[6];
+};
+// That of a pick workgroup: where no row filters, and where rows may.
+struct DrawShared {
+  static constexpr int NW = kWaves;
+  double red[NW];
+  double logz;
+  int i[2];
+};
 struct PickShared {
+  static constexpr int NW = kWaves;
   u32x4 ring[kWaves * kAhead * 64];
   uint64_t raw[kList];     // ranks as collected
   uint64_t sorted[kList];  // ranks, earliest first
   uint32_t bin[kBins];     // counts or weights
-  double red[kWaves];
-  uint32_t cnt[kWaves];
+  double red[NW];
+  uint32_t cnt[NW];
+  double logz;
   int n;
   int i[8];
 };
 
 // The sum over the workgroup, the same bits in every thread.
-__device__ __forceinline__ double block_sum(PickShared& sh, double v) {
+template <class SH>
+__device__ __forceinline__ double block_sum(SH& sh, double v) {
   v = wave_sum(v);
   __syncthreads();
   if ((item_id() & 63) == 0) sh.red[item_id() >> 6] = v;
   __syncthreads();
   double t = 0.0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) t += sh.red[w];
+  for (int w = 0; w < SH::NW; ++w) t += sh.red[w];
   return t;
 }
 // Exclusive prefix sum over the workgroup's threads, and the whole sum.
-__device__ __forceinline__ double block_scan(PickShared& sh, double v, double* total) {
+template <class SH>
+__device__ __forceinline__ double block_scan(SH& sh, double v, double* total) {
   const int wave = item_id() >> 6;
   double mine;
   const double e = wave_scan(v, &mine);
@@ -344,7 +374,7 @@ __device__ __forceinline__ double block_scan(PickShared& sh, double v, double* t
   __syncthreads();
   double before = 0.0, t = 0.0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < SH::NW; ++w) {
     if (w == wave) before = t;
     t += sh.red[w];
   }
@@ -362,6 +392,23 @@ __device__ __forceinline__ uint32_t block_reduce_u32(PickShared& sh, uint32_t v,
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) t = f(t, sh.cnt[w]);
   return t;
+}
+// The smallest of the threads' `lo` (their wave first: a thousand atomics on one word took 17 us)
+// and the largest of their `hi`, in sh.i[at] and sh.i[at + 1].
+template <class SH>
+__device__ __forceinline__ void block_min_max(SH& sh, int at, int lo, int hi) {
+  if (item_id() == 0) {
+    sh.i[at] = 0x7fffffff;
+    sh.i[at + 1] = -0x7fffffff;
+  }
+  __syncthreads();
+  lo = wave_min(lo);
+  hi = wave_max(hi);
+  if ((item_id() & 63) == 0) {
+    atomicMin(&sh.i[at], lo);
+    atomicMax(&sh.i[at + 1], hi);
+  }
+  __syncthreads();
 }
 
 // Descending bitonic sort of v[0 .. n), padded with zeros to a power of two (at most kList).
@@ -954,18 +1001,81 @@ __device__ __forceinline__ float list_bound(const float* gm, int n, int k) {
   return of_key(lo);
 }
 
+// A row's largest logit, and its weight against that; each wave by itself.
+__device__ __forceinline__ float row_max(const SampleParams& p, int row) {
+  const float* gm = p.gmax + (int64_t)row * p.groups;
+  float m = kNegInf;
+#pragma unroll 2
+  for (int g = item_id() & 63; g < p.groups; g += 64) m = fmaxf(m, gm[g]);
+  return wave_max_all(m);
+}
+__device__ __forceinline__ double row_weight(const SampleParams& p, int row, float m, double inv2) {
+  const int64_t at = (int64_t)row * p.groups;
+  double w = 0.0;
+#pragma unroll 1
+  for (int g = item_id() & 63; g < p.groups; g += 64)
+    w += p.sum_t[at + g] * weight(p.gmax[at + g], m, inv2);
+  return wave_sum(w);
+}
+
+// A nucleus' histogram: bins of equal steps of the weight's logarithm below the maximum, weights as
+// integers of f32 exponentials whose sum over the row stays below 2^31 (adding them in any order
+// gives the same sum). They reach as far as the boundary may lie: n tokens of weight below
+// (1 - p) W / n weigh less than (1 - p) W together, and none below min_p is kept.
+struct CutBins {
+  float m = 0.f, scale = 0.f, inv2f = 0.f;
+  int wshift = 0;
+  CutBins() = default;
+  __device__ __forceinline__ CutBins(float m, const RowSettings& s, int n, double whole) : m(m) {
+    double reach = s.mp > 0.0 ? -log2(s.mp) : log2((double)n / ((1.0 - (double)s.p) * whole));
+    reach = __builtin_fmin(__builtin_fmax(reach + 0.25, 1.0), 64.0);
+    scale = fminf((float)(s.inv2 * (kCutBins / reach)), 1e30f);
+    inv2f = fminf((float)s.inv2, 1e30f);
+    wshift = 30 - (int)__builtin_ceil(log2(fmax(whole, 1.0)));
+  }
+  // a bin where below kCutBins; it does not fall as logits do
+  __device__ __forceinline__ float pos(float l) const {
+    return l >= m ? 0.f : fminf((m - l) * scale, (float)kCutBins);
+  }
+  __device__ __forceinline__ uint32_t value(float l) const {
+    const float wscale = __builtin_ldexpf(1.f, wshift);
+    return (uint32_t)(l >= m ? wscale : fast_exp2((l - m) * inv2f) * wscale);
+  }
+};
+
+// Sums over the groups of a chunk from those of the waves' loads: entry n covers elements
+// n * 64 EPL on. Called by the workgroup's first threads.
+template <int EPL>
+__device__ __forceinline__ void put_group_sums(const SampleParams& p, double* to, int row, int chunk,
+                                               const double* red) {
+  constexpr int PER = kGroup / (64 * EPL), N = kChunk / kGroup;
+  const int t = item_id(), g = chunk * N + t;
+  if (t >= N || g >= p.groups) return;
+  double x = 0.0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) x += red[t * PER + j];
+  to[(int64_t)row * p.groups + g] = x;
+}
+
 template <int DT, bool TINY>
-__global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p, int per) {
+__global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
   constexpr int EPL = Lane<DT, TINY>::EPL, IT = kChunk / (256 * EPL);
   constexpr int kHeld = 1024;  // maxima at most
-  __shared__ float bound;
+  __shared__ float bound, top;
+  __shared__ double whole;
   __shared__ int count[2];
+  __shared__ double red[2][kChunk / (64 * EPL)];
+  __shared__ __attribute__((aligned(16))) uint32_t hist[kCutBins];
   const int row = wg_id_y(), tid = item_id(), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const RowSettings s = settings(p, row);
   if (s.greedy || !s.filtered()) return;
+  bool nucleus = s.k == 0 && s.p < 1.f;
+  const bool minima = s.k == 0 && s.mp > 0.0;
   const ListRule rule = list_rule(s, p.groups);
-  const int c0 = wg_id_x() * per, c1 = min(c0 + per, p.chunks);
-  if (rule.n == 0 || rule.n > kHeld) {
+  const bool listing = rule.n > 0 && rule.n <= kHeld;
+  const int c0 = wg_id_x() * p.per, c1 = min(c0 + p.per, p.chunks);
+  if (!listing && !nucleus && !minima) {
     if (c0 == 0 && tid == 0) p.low[row] = kNegInf;
     return;
   }
@@ -975,21 +1085,72 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p, int 
   for (int i = 0; i < IT; ++i)
     a[i] = Lane<DT, TINY>::raw(x, c0 * kChunk + (i * 256 + tid) * EPL, p.vocab);
   if (tid < 2) count[tid] = 0;
-  if (tid < 64) {
-    const float* gm = rule.fine ? p.smax + (int64_t)row * p.groups * 4 : p.gmax + (int64_t)row * p.groups;
-    const float b = rule.n <= 128   ? list_bound<2>(gm, rule.n, rule.k)
-                    : rule.n <= 256 ? list_bound<4>(gm, rule.n, rule.k)
-                                    : list_bound<kHeld / 64>(gm, rule.n, rule.k);
+  if (nucleus)
+    for (int b = tid; b < kCutBins; b += 256) hist[b] = 0;
+  if (wave == 0) {
+    float b = kNegInf;
+    if (listing) {
+      const float* gm =
+          rule.fine ? p.smax + (int64_t)row * p.groups * 4 : p.gmax + (int64_t)row * p.groups;
+      b = rule.n <= 128   ? list_bound<2>(gm, rule.n, rule.k)
+          : rule.n <= 256 ? list_bound<4>(gm, rule.n, rule.k)
+                          : list_bound<kHeld / 64>(gm, rule.n, rule.k);
+    }
     if (lane == 0) bound = b;
+  } else if (wave == 1 && (nucleus || minima)) {
+    const float m = row_max(p, row);
+    const double w = nucleus && m != kNegInf ? row_weight(p, row, m, s.inv2) : 0.0;
+    if (lane == 0) {
+      top = m;
+      whole = w;
+    }
   }
   __syncthreads();
   const float low = bound;
   if (c0 == 0 && tid == 0) p.low[row] = low;
-  if (low == kNegInf) return;
+  if (low == kNegInf && !nucleus && !minima) return;
+  const float m = nucleus || minima ? top : 0.f;
+  if (m == kNegInf) return;
+  nucleus = nucleus && m != __builtin_inff();
+  CutBins bins;
+  if (nucleus) bins = CutBins(m, s, p.vocab, whole);
+  const float inv2f = fminf((float)s.inv2, 1e30f);
+  // (surely below min_p: no f64 weight)
+  float min_y = 0.f;
+  if (minima) min_y = (float)log2(s.mp) - 0.01f;
 #pragma unroll 1
   for (int c = c0; c < c1; ++c) {
     uint64_t* to = p.cand + ((int64_t)row * p.chunks + c) * kShort;
     int* n = &count[c & 1];
+    if (nucleus || minima) {
+      // (a loop of one load, from the caches: the code is there once)
+#pragma unroll 1
+      for (int i = 0; i < IT; ++i) {
+        const int i0 = c * kChunk + (i * 256 + tid) * EPL;
+        Lane<DT, TINY> cur;
+        cur.take(Lane<DT, TINY>::raw(x, i0, p.vocab), i0, p.vocab, p.vocab,
+                 c * kChunk + (i + 1) * 256 * EPL);
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+          const float l = cur.v[e];
+          if (nucleus) {
+            const float at = bins.pos(l);
+            if (at < (float)kCutBins) atomicAdd(&hist[(int)at], bins.value(l));
+          }
+          if (minima) {
+            if (__ballot(l >= m || (l - m) * inv2f >= min_y)) {
+              const double w = weight(l, m, s.inv2);
+              sum += w >= s.mp ? w : 0.0;
+            }
+          }
+        }
+        if (minima) {
+          sum = wave_sum(sum);
+          if (lane == 0) red[c & 1][i * 4 + wave] = sum;
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int i0 = c * kChunk + (i * 256 + tid) * EPL;
@@ -998,7 +1159,7 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p, int 
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
         const float l = cur.v[e];
-        const bool take = l >= low;
+        const bool take = l >= low && low != kNegInf;
         const uint64_t v = __ballot(take);
         if (v == 0) continue;  // uniform
         int at = 0;
@@ -1010,39 +1171,338 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p, int 
       a[i] = Lane<DT, TINY>::raw(x, i0 + kChunk, p.vocab);
     }
     __syncthreads();
+    // (the next chunk uses the other word and row, and its barrier comes before these ones' reuse)
     if (tid == 0) {
       p.count[(int64_t)row * p.chunks + c] = *n;
-      *n = 0;  // (the next chunk counts in the other word, and its barrier comes before this one's reuse)
+      *n = 0;
     }
+    if (minima) put_group_sums<EPL>(p, p.sum_k, row, c, red[c & 1]);
+  }
+  if (nucleus) {
+    u32x4* to = reinterpret_cast<u32x4*>(p.hist + ((int64_t)row * p.parts + wg_id_x()) * kCutBins);
+    for (int b = tid; b < kCutBins / 4; b += 256) to[b] = reinterpret_cast<const u32x4*>(hist)[b];
   }
 }
 
 // ---- pick --------------------------------------------------------------------------------------
+// The token by the groups' weights: the group that holds u times the whole (each wave by itself),
+// then its elements, one a thread. sums(g): a group's weight; keep(i, l): an element's.
 static_assert(kGroup == kPick, "one element of a group per thread");
+template <int DT, class SH, class F, class G>
+__device__ __forceinline__ int draw_groups(SH& sh, const store_t<DT>* x, int vocab, int groups,
+                                           double u, F sums, G keep) {
+  const int tid = item_id(), lane = tid & 63;
+  if (tid == 0) {
+    sh.i[0] = 0x7fffffff;
+    sh.i[1] = 0;
+  }
+  // lane: the groups from lane * per
+  const int per = (groups + 63) / 64, g0 = lane * per, g1 = min(g0 + per, groups);
+  double mine = 0.0, total;
+#pragma unroll 1
+  for (int g = g0; g < g1; ++g) mine += sums(g);
+  double run = wave_scan(mine, &total);
+  const double target = u * total;
+  const uint64_t pass = __ballot(mine > 0.0 && run + mine > target);
+  const uint64_t any = __ballot(mine > 0.0);
+  const int who = pass ? __builtin_ctzll(pass) : any ? 63 - __builtin_clzll(any) : 0;
+  int g_hit = 0;
+  double left = 0.0;
+  if (per == 1) {
+    g_hit = lane;
+    left = target - run;
+  } else if (lane == who) {
+    bool done = false;
+#pragma unroll 1
+    for (int g = g0; g < g1; ++g) {
+      const double w = sums(g);
+      if (!done && w > 0.0) {  // (the last one of any weight where rounding leaves none)
+        g_hit = g;
+        left = target - run;
+        done = run + w > target;
+      }
+      run += w;
+    }
+  }
+  g_hit = __builtin_amdgcn_readfirstlane(__shfl(g_hit, who));
+  left = __shfl(left, who);
+  const int i = g_hit * kGroup + tid;
+  const double w = i < vocab ? keep(i, load1<DT>(x, i)) : 0.0;
+  run = block_scan(sh, w, &total);
+  const int hit = wave_min(w > 0.0 && run + w > left ? i : 0x7fffffff);
+  const int last = wave_max(w > 0.0 ? i : 0);
+  if (lane == 0) {
+    atomicMin(&sh.i[0], hit);
+    atomicMax(&sh.i[1], last);
+  }
+  __syncthreads();
+  return sh.i[0] != 0x7fffffff ? sh.i[0] : sh.i[1];
+}
 
+// Collects a row's listed ranks, `held` at most (first: the lane's chunk's count); how many there are (more where a chunk's list is cut).
+template <class SH>
+__device__ __forceinline__ int collect(SH& sh, const int32_t* counts, int first,
+                                       const uint64_t* cand, int chunks, int held) {
+  const int lane = item_id() & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(item_id() >> 6);
+  // chunk counts by lane (every wave alike), places by their running sum
+  int n = 0;
+  bool over = false;
+  for (int c0 = 0; c0 < chunks; c0 += 64) {
+    const int c = c0 + lane >= chunks ? 0 : c0 == 0 ? first : counts[c0 + lane];
+    over = over || __ballot(c > kShort) != 0;
+    int before = c;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int y = __shfl_up(before, d);
+      if (lane >= d) before += y;
+    }
+    const int all = __shfl(before, 63);
+    before += n - c;
+    // waves take the chunks in turn
+    for (int j = wave; j < min(64, chunks - c0); j += SH::NW) {
+      const int cj = min(__shfl(c, j), kShort), at0 = __shfl(before, j);
+      const uint64_t* from = cand + (int64_t)(c0 + j) * kShort;
+      for (int q = lane; q < cj; q += 64)
+        if (at0 + q < held) sh.raw[at0 + q] = from[q];
+    }
+    n += all;
+  }
+  __syncthreads();
+  return over ? max(n, held + 1) : n;
+}
+
+// Whether the gathered list (from `low` on) settles the row: sh.raw[0 .. *n), and W(S1) in *whole where
+// S1 reaches below the list (else -1). first: the count of chunk `lane`.
+template <class SH>
+__device__ __forceinline__ bool settled(const SampleParams& p, SH& sh, int row, const RowSettings& s,
+                                        float low, int first, float m, double W, int* n,
+                                        double* whole) {
+  *whole = -1.0;
+  if (low == kNegInf) return false;
+  *n = collect(sh, p.count + (int64_t)row * p.chunks, first, p.cand + (int64_t)row * p.chunks * kShort,
+               p.chunks, kShort);
+  if (*n > kShort) return false;
+  // every kept token is listed when the k-th, the least weight or the limit ends inside
+  if (s.k > 0 || (s.mp > 0.0 && weight(low, m, s.inv2) < s.mp)) return true;
+  if (s.mp > 0.0 || s.p >= 1.f) return false;
+  const int tid = item_id();
+  double x = tid < *n ? weight(logit_of(sh.raw[tid]), m, s.inv2) : 0.0;
+  x = block_sum(sh, x);
+  *whole = W;
+  // (a limit so near the list's end that rounding decides goes the long way)
+  return x * (1.0 - 1e-12) >= (double)s.p * W;
+}
+
+// An open nucleus, spread over the row's chunks: the bins of the histogram that the limit may lie
+// in, by as much as its integers may be off; the tokens in them are listed, the weights above them
+// summed by group; the pick finishes the row.
 template <int DT, bool TINY>
+__global__ __launch_bounds__(kSpread) void sample_spread_kernel(SampleParams p) {
+  constexpr int EPL = Lane<DT, TINY>::EPL, IT = kChunk / (kSpread * EPL);
+  __shared__ SpreadShared sh;
+  const int part = wg_id_x(), row = wg_id_y();
+  const int tid = item_id(), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const RowSettings s = settings(p, row);
+  if (s.greedy || s.k > 0 || s.p >= 1.f) return;
+  const float low = p.low[row];
+  const int first = p.count[(int64_t)row * p.chunks + min(lane, p.chunks - 1)];
+  const float m = row_max(p, row);
+  if (m == kNegInf) return;
+  const double W = row_weight(p, row, m, s.inv2);
+  int n;
+  double w1;
+  if (m == __builtin_inff() || settled(p, sh, row, s, low, first, m, W, &n, &w1)) {
+    if (part == 0 && tid == 0) p.cut[row] = 0;
+    return;
+  }
+  w1 = W;
+  if (s.mp > 0.0) {  // W(S1)
+    w1 = 0.0;
+#pragma unroll 1
+    for (int g = lane; g < p.groups; g += 64) w1 += p.sum_k[(int64_t)row * p.groups + g];
+    w1 = wave_sum(w1);
+  }
+  const double want = (double)s.p * w1;
+  const CutBins bins(m, s, p.vocab, W);
+  // ---- thread t: bins PB t ..
+  constexpr int PB = kCutBins / kSpread;
+  static_assert(PB == 4, "a 16-byte load of bins");
+  u32x4 c = {0u, 0u, 0u, 0u};
+  {
+    const u32x4* h = reinterpret_cast<const u32x4*>(p.hist + (int64_t)row * p.parts * kCutBins) + tid;
+#pragma unroll 4
+    for (int j = 0; j < p.parts; ++j) c += h[(int64_t)j * (kCutBins / 4)];
+  }
+  double w[PB], sum = 0.0, total;
+#pragma unroll
+  for (int e = 0; e < PB; ++e) {
+    w[e] = __builtin_ldexp((double)c[e], -bins.wshift);
+    sum += w[e];
+  }
+  double run = block_scan(sh, sum, &total);
+  // (an integer weight is truncated: one step an element)
+  const double slack = total * 0x1p-17 + __builtin_ldexp((double)p.vocab, -bins.wshift);
+  int b0 = kCutBins, b1 = kCutBins;
+#pragma unroll
+  for (int e = 0; e < PB; ++e) {
+    run += w[e];
+    if (run >= want - slack) b0 = min(b0, PB * tid + e);
+    if (run >= want + slack) b1 = min(b1, PB * tid + e);
+  }
+  block_min_max(sh, 0, b0, -b1);
+  const int lo = sh.i[0], hi = -sh.i[1];
+  if (part == 0 && tid == 0) p.cut[row] = hi < kCutBins ? 1 : 0;
+  if (hi >= kCutBins) return;
+  // ---- the logits at the bins' ends, by bisection: the least key of bins [0, lo - 1] (lanes 0 ..
+  // 31) and of bins [0, hi]
+  uint32_t kx = key_of(kNegInf) + 1, ky = key_of(m);
+  {
+    const float b = (float)(lane < 32 ? lo : hi + 1);
+    while (__ballot(kx < ky)) {
+      const uint32_t mid = kx + (ky - kx) / 2;
+      if (kx < ky) {
+        if (bins.pos(of_key(mid)) < b) ky = mid;
+        else kx = mid + 1;
+      }
+    }
+  }
+  const uint32_t k_lo = (uint32_t)__shfl((int)kx, 0), k_hi = (uint32_t)__shfl((int)kx, 32);
+  const float ftop = lo == 0 ? m : of_key(k_lo - 1), fbottom = of_key(k_hi);
+  // ---- list what the bins hold, sum what lies above them
+  const store_t<DT>* x = reinterpret_cast<const store_t<DT>*>(p.logits) + (int64_t)row * p.ls;
+  const int c0 = part * p.per, c1 = min(c0 + p.per, p.chunks);
+  int* count = &sh.i[4];  // two, by turns
+  u32x4 r[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i)
+    r[i] = Lane<DT, TINY>::raw(x, c0 * kChunk + (i * kSpread + tid) * EPL, p.vocab);
+  if (tid < 2) count[tid] = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int ch = c0; ch < c1; ++ch) {
+    uint64_t* to = p.cand2 + ((int64_t)row * p.chunks + ch) * kShort;
+    int* held = &count[ch & 1];
+    double* rd = sh.sums[ch & 1];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int i0 = ch * kChunk + (i * kSpread + tid) * EPL;
+      Lane<DT, TINY> cur;
+      cur.take(r[i], i0, p.vocab, p.vocab, ch * kChunk + (i + 1) * kSpread * EPL);
+      double above = 0.0;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float l = cur.v[e];
+        const bool take = l >= fbottom && l <= ftop;
+        const uint64_t v = __ballot(take);
+        if (v != 0) {  // uniform
+          int at = 0;
+          if (lane == 0) at = atomicAdd(held, __popcll(v));
+          at = __builtin_amdgcn_readfirstlane(at) + __popcll(v & ((uint64_t(1) << lane) - 1));
+          if (take && at < kShort) to[at] = rank_of(l, i0 + e);
+        }
+        if (__ballot(l > ftop)) above += l > ftop ? weight(l, m, s.inv2) : 0.0;
+      }
+      r[i] = Lane<DT, TINY>::raw(x, i0 + kChunk, p.vocab);
+      above = wave_sum(above);
+      if (lane == 0) rd[i * SpreadShared::NW + wave] = above;
+    }
+    __syncthreads();
+    // (the next chunk uses the other word and row, and its barrier comes before these ones' reuse)
+    if (tid == 0) {
+      p.count2[(int64_t)row * p.chunks + ch] = *held;
+      *held = 0;
+    }
+    put_group_sums<EPL>(p, p.sum_a, row, ch, rd);
+  }
+}
+
+// A nucleus whose boundary's bins are listed (n tokens, sh.raw): ordered, the definition applied;
+// then the token by the groups' weights.
+template <int DT, bool TINY>
+__device__ __forceinline__ int finish_cut(const SampleParams& p, const Row<DT, TINY>& row,
+                                          PickShared& sh, int rowi, int n, const RowSettings& s,
+                                          float m, double W, double u) {
+  const int tid = item_id(), lane = tid & 63;
+  const int64_t at = (int64_t)rowi * p.groups;
+  double above = 0.0, w1 = W;
+  if (s.mp > 0.0) w1 = 0.0;
+#pragma unroll 1
+  for (int g = lane; g < p.groups; g += 64) {
+    above += p.sum_a[at + g];
+    if (s.mp > 0.0) w1 += p.sum_k[at + g];
+  }
+  above = wave_sum(above);
+  if (s.mp > 0.0) w1 = wave_sum(w1);
+  const double want = (double)s.p * w1;
+  for (int j = tid; j < n; j += kPick) sh.sorted[j] = sh.raw[j];
+  __syncthreads();
+  sort_list(sh.sorted, n);
+  constexpr int PL = kList / kPick;
+  double w[PL], mine = 0.0, total;
+#pragma unroll
+  for (int e = 0; e < PL; ++e) {
+    w[e] = PL * tid + e < n ? weight(logit_of(sh.sorted[PL * tid + e]), m, s.inv2) : 0.0;
+    mine += w[e];
+  }
+  double before = above + block_scan(sh, mine, &total);
+  int last = 0;
+#pragma unroll
+  for (int e = 0; e < PL; ++e) {
+    if (PL * tid + e < n && before < want) last = PL * tid + e;
+    before += w[e];
+  }
+  block_min_max(sh, 0, 0, last);
+  last = sh.i[1];
+  const uint64_t low = sh.sorted[last];
+  // the listed tokens that are kept join their groups, as multiples of 2^-52 of the largest weight
+  // (adding integers in any order gives the same sum)
+  uint64_t* sums = reinterpret_cast<uint64_t*>(sh.ring);
+  for (int g = tid; g < p.groups; g += kPick) sums[g] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < PL; ++e) {
+    const int j = PL * tid + e;
+    if (j <= last)
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sums[index_of(sh.sorted[j]) / kGroup]),
+                (unsigned long long)(w[e] * 0x1p52));
+  }
+  __syncthreads();
+  return draw_groups<DT>(
+      sh, row.x, p.vocab, p.groups, u, [&](int g) { return p.sum_a[at + g] + (double)sums[g] * 0x1p-52; },
+      [&](int i, float l) { return rank_of(l, i) >= low ? weight(l, m, s.inv2) : 0.0; });
+}
+static_assert(sizeof(PickShared::ring) >= kMaxVocab / kGroup * sizeof(double), "a sum per group");
+
+// FILTER: rows may filter. (Without, a kernel of a tenth of the code, which comes cold from memory.)
+template <int DT, bool TINY, bool FILTER>
 __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) char pick_lds[];
-  PickShared& sh = *reinterpret_cast<PickShared*>(pick_lds);
+  using SH = std::conditional_t<FILTER, PickShared, DrawShared>;
+  SH& sh = *reinterpret_cast<SH*>(pick_lds);
   const int rowi = wg_id_x(), tid = item_id(), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Row<DT, TINY> row;
   row.x = reinterpret_cast<const store_t<DT>*>(p.logits) + (int64_t)rowi * p.ls;
   row.n = p.vocab;
-  row.ring = sh.ring;
+  if constexpr (FILTER) row.ring = sh.ring;
   const RowSettings s = settings(p, rowi);
-  const bool simple = s.greedy || !s.filtered();
   if (s.greedy && wave > 0) return;  // one wave's work, no barrier
   const float uf = p.u[rowi];
   const double u = is_nan(uf) || uf < 0.f ? 0.0 : (double)fminf(uf, 0x1.fffffep-1f);
-
-  // ---- the row's maximum, in every wave (lane: groups lane, lane + 64, ..)
   const int64_t at = (int64_t)rowi * p.groups;
   const float* gm = p.gmax + at;
-  float m = kNegInf;
-#pragma unroll 2
-  for (int g = lane; g < p.groups; g += 64) m = fmaxf(m, gm[g]);
-  m = wave_max_all(m);
+  // (on their way while the maximum is found; of rows that filter, the list's bound and counts)
+  const int first = min(lane, p.groups - 1);
+  const double sum_1 = p.sum_1[at + first], sum_t = p.sum_t[at + first];
+  float low = kNegInf;
+  int count = 0;
+  if constexpr (FILTER) {
+    low = p.low[rowi];
+    count = p.count[(int64_t)rowi * p.chunks + min(lane, p.chunks - 1)];
+  }
+  const float m = row_max(p, rowi);
   if (m == kNegInf) {  // nothing to choose from (uniform)
     if (tid == 0) {
       p.tok[rowi] = -1;
@@ -1050,13 +1510,14 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     }
     return;
   }
-  // log of the row's sum at temperature 1 (m apart), wave 0
-  double logz = 0.0;
-  if (wave == 0 && p.lp) {
+  // log of the row's sum at temperature 1 (m apart): the last wave's, beside the others' work
+  if (p.lp && (s.greedy || wave == kWaves - 1)) {
     double r = 0.0;
 #pragma unroll 1
-    for (int g = lane; g < p.groups; g += 64) r += p.sum_1[at + g] * weight(gm[g], m, kLog2e);
-    logz = log(wave_sum(r));
+    for (int g = lane; g < p.groups; g += 64)
+      r += (g == lane ? sum_1 : p.sum_1[at + g]) * weight(gm[g], m, kLog2e);
+    r = log(wave_sum(r));
+    if (lane == 0) sh.logz = r;
   }
   int token = 0;
   if (s.greedy) {
@@ -1077,110 +1538,46 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         if (a.v[e] == m) f = i + e;
     }
     token = wave_min(f);
-  } else if (simple) {
-    // lane: the groups from lane * per; the group that passes u W, then its 1024 elements
-    const int per = (p.groups + 63) / 64, g0 = lane * per;
-    double mine = 0.0, total;
-#pragma unroll 1
-    for (int g = g0; g < min(g0 + per, p.groups); ++g)
-      mine += p.sum_t[at + g] * weight(gm[g], m, s.inv2);
-    double run = wave_scan(mine, &total);
-    const double target = u * total;
-    const uint64_t pass = __ballot(mine > 0.0 && run + mine > target);
-    const uint64_t any = __ballot(mine > 0.0);
-    const int who = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(any);
-    int g_hit = 0;
-    double left = 0.0;
-    if (lane == who) {
-      bool done = false;
-#pragma unroll 1
-      for (int g = g0; g < min(g0 + per, p.groups); ++g) {
-        const double w = p.sum_t[at + g] * weight(gm[g], m, s.inv2);
-        if (!done && w > 0.0) {  // (the last one of any weight where rounding leaves none)
-          g_hit = g;
-          left = target - run;
-          done = run + w > target;
-        }
-        run += w;
+  } else if (!FILTER || !s.filtered()) {
+    token = draw_groups<DT>(
+        sh, row.x, p.vocab, p.groups, u,
+        [&](int g) {
+          return (p.groups <= 64 ? sum_t : p.sum_t[at + g]) * weight(gm[g], m, s.inv2);
+        },
+        [&](int, float l) { return weight(l, m, s.inv2); });
+  } else if constexpr (FILTER) {
+    const double W = s.k == 0 ? row_weight(p, rowi, m, s.inv2) : 0.0;
+    int n = 0;
+    double whole = -1.0;
+    if (settled(p, sh, rowi, s, low, count, m, W, &n, &whole)) {
+      token = pick_short(sh, n, s, m, whole, u);
+    } else if (s.k == 0 && s.p >= 1.f) {
+      // the tokens of weight >= min_p
+      token = draw_groups<DT>(
+          sh, row.x, p.vocab, p.groups, u, [&](int g) { return p.sum_k[at + g]; },
+          [&](int, float l) {
+            const double w = weight(l, m, s.inv2);
+            return w >= s.mp ? w : 0.0;
+          });
+    } else {
+      n = kList + 1;
+      if (s.k == 0 && p.cut[rowi] != 0) {
+        __syncthreads();  // (the list that did not settle it is done with)
+        const int32_t* counts = p.count2 + (int64_t)rowi * p.chunks;
+        n = collect(sh, counts, counts[min(lane, p.chunks - 1)],
+                    p.cand2 + (int64_t)rowi * p.chunks * kShort, p.chunks, kList);
       }
+      token = n > 0 && n <= kList ? finish_cut(p, row, sh, rowi, n, s, m, W, u)
+                                  : pick_wide(row, sh, s, m, W, u);
     }
-    g_hit = __shfl(g_hit, who);
-    left = __shfl(left, who);
-    // the group's elements, one a thread (kGroup == kPick)
-    const int i = g_hit * kGroup + tid;
-    const double w = i < row.n ? weight(load1<DT>(row.x, i), m, s.inv2) : 0.0;
-    run = block_scan(sh, w, &total);
-    if (tid == 0) {
-      sh.i[0] = 0x7fffffff;
-      sh.i[1] = 0;
-    }
-    __syncthreads();
-    const int hit = wave_min(w > 0.0 && run + w > left ? i : 0x7fffffff);
-    const int lastk = wave_max(w > 0.0 ? i : 0);
-    if (lane == 0) {
-      atomicMin(&sh.i[0], hit);
-      atomicMax(&sh.i[1], lastk);
-    }
-    __syncthreads();
-    token = sh.i[0] != 0x7fffffff ? sh.i[0] : sh.i[1];
-  } else {
-    double W = 0.0;
-    if (s.k == 0) {
-#pragma unroll 1
-      for (int g = lane; g < p.groups; g += 64) W += p.sum_t[at + g] * weight(gm[g], m, s.inv2);
-      W = wave_sum(W);
-    }
-    // ---- the gathered list (the rule that made it says whether there is one)
-    bool done = false;
-    const ListRule rule = list_rule(s, p.groups);
-    const float low = rule.n == 0 ? kNegInf : p.low[rowi];
-    if (low != kNegInf) {
-      // chunk counts by lane (every wave alike), places by their running sum
-      const int32_t* counts = p.count + (int64_t)rowi * p.chunks;
-      int n = 0;
-      for (int c0 = 0; c0 < p.chunks; c0 += 64) {
-        const int c = c0 + lane < p.chunks ? counts[c0 + lane] : 0;
-        int before = c;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const int y = __shfl_up(before, d);
-          if (lane >= d) before += y;
-        }
-        const int all = __shfl(before, 63);
-        before += n - c;
-        // waves take the chunks in turn
-        for (int j = wave; j < min(64, p.chunks - c0); j += kWaves) {
-          const int cj = min(__shfl(c, j), kShort), at0 = __shfl(before, j);
-          const uint64_t* from = p.cand + ((int64_t)rowi * p.chunks + c0 + j) * kShort;
-          for (int q = lane; q < cj; q += 64)
-            if (at0 + q < kShort) sh.raw[at0 + q] = from[q];
-        }
-        n += all;
-      }
-      __syncthreads();
-      if (n <= kShort) {
-        // every kept token is listed when the k-th, the least weight or the limit ends inside
-        const bool by_mp = s.mp > 0.0 && weight(low, m, s.inv2) < s.mp;
-        double whole = -1.0;
-        done = s.k > 0 || by_mp;
-        if (!done && s.mp <= 0.0 && s.p < 1.f) {
-          double x = tid < n ? weight(logit_of(sh.raw[tid]), m, s.inv2) : 0.0;
-          x = block_sum(sh, x);
-          // (a limit so near the list's end that rounding decides goes the wide way)
-          done = x * (1.0 - 1e-12) >= (double)s.p * W;
-          whole = W;
-        }
-        if (done) token = pick_short(sh, n, s, m, whole, u);
-      }
-    }
-    if (!done) token = pick_wide(row, sh, s, m, W, u);
   }
+  // (every way here but the greedy one has passed barriers since sh.logz was written)
   if (tid == 0) {
     p.tok[rowi] = token;
     if (p.lp) {
       const float l = load1<DT>(row.x, token);
       const double d = l >= m ? 0.0 : (double)l - (double)m;
-      p.lp[rowi] = (float)(d - logz);
+      p.lp[rowi] = (float)(d - sh.logz);
     }
   }
 }
@@ -1188,19 +1585,26 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
 template <int DT, bool TINY>
 hipError_t launch_sample(const SampleParams& p, hipStream_t st) {
   static const hipError_t once = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(sample_pick_kernel<DT, TINY>),
+      reinterpret_cast<const void*>(sample_pick_kernel<DT, TINY, true>),
       hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PickShared));
   if (once != hipSuccess) return once;
-  hipLaunchKernelGGL((sample_scan_kernel<DT, TINY>), dim3((unsigned)((p.groups + 3) / 4), (unsigned)p.rows), dim3(256), 0,
-                     st, p);
-  if (p.k || p.k_all > 0 || p.p || p.p_all < 1.f || p.mp || p.mp_all > 0.f) {  // a row may filter
-    // four chunks a workgroup where that leaves enough of them: each finds the row's bound by itself
-    const int per = (int64_t)p.chunks * p.rows >= 4096 ? 4 : 1;
-    hipLaunchKernelGGL((sample_gather_kernel<DT, TINY>),
-                       dim3((unsigned)((p.chunks + per - 1) / per), (unsigned)p.rows), dim3(256), 0,
-                       st, p, per);
+  const unsigned rows = (unsigned)p.rows;
+  // what rows may do, as far as the host knows
+  const bool counts = p.k || p.k_all > 0, nuclei = p.p || p.p_all < 1.f;
+  const bool minima = p.mp || p.mp_all > 0.f, all_count = !p.k && p.k_all > 0 && p.k_all < p.vocab;
+  hipLaunchKernelGGL((sample_scan_kernel<DT, TINY>), dim3((unsigned)((p.groups + 3) / 4), rows),
+                     dim3(256), 0, st, p);
+  if (!counts && !nuclei && !minima) {
+    hipLaunchKernelGGL((sample_pick_kernel<DT, TINY, false>), dim3(rows), dim3(kPick),
+                       sizeof(DrawShared), st, p);
+    return hipGetLastError();
   }
-  hipLaunchKernelGGL((sample_pick_kernel<DT, TINY>), dim3((unsigned)p.rows), dim3(kPick), sizeof(PickShared),
+  hipLaunchKernelGGL((sample_gather_kernel<DT, TINY>), dim3((unsigned)p.parts, rows), dim3(256), 0, st,
+                     p);
+  if (nuclei && !all_count)
+    hipLaunchKernelGGL((sample_spread_kernel<DT, TINY>), dim3((unsigned)p.parts, rows), dim3(kSpread),
+                       0, st, p);
+  hipLaunchKernelGGL((sample_pick_kernel<DT, TINY, true>), dim3(rows), dim3(kPick), sizeof(PickShared),
                      st, p);
   return hipGetLastError();
 }
@@ -1210,13 +1614,22 @@ int check_sample_sizes(int32_t rows, int32_t vocab) {
   if (vocab < 1 || vocab > kMaxVocab) return api_fail(FFAI_ERR_INVALID, "vocab must be in [1, 2^20]");
   return FFAI_OK;
 }
+// Chunks of a gather workgroup: four where that leaves enough of them (each finds the row's bound by
+// itself), and so many that a row has kParts at most (a nucleus reads all their histograms).
+int32_t sample_per(int32_t rows, int32_t chunks) {
+  const int32_t per = (int64_t)chunks * rows >= 4096 ? 4 : 1;
+  return std::max(per, (chunks + kParts - 1) / kParts);
+}
 // The workspace's parts, in order, each 16-byte aligned.
 struct SampleSpace {
-  size_t sum_t, sum_1, cand, gmax, smax, low, count, bytes;
+  size_t sum_t, sum_1, sum_k, sum_a, cand, cand2, hist, gmax, smax, low, count, count2, cut,
+      bytes;
 };
 SampleSpace sample_space(int32_t rows, int32_t vocab) {
   const size_t g = (size_t)rows * ((vocab + kGroup - 1) / kGroup);
-  const size_t c = (size_t)rows * ((vocab + kChunk - 1) / kChunk);
+  const int32_t chunks = (vocab + kChunk - 1) / kChunk;
+  const size_t c = (size_t)rows * chunks;
+  const int32_t per = sample_per(rows, chunks);
   SampleSpace s{};
   auto take = [&](size_t n) {
     const size_t at = s.bytes;
@@ -1225,11 +1638,17 @@ SampleSpace sample_space(int32_t rows, int32_t vocab) {
   };
   s.sum_t = take(g * 8);
   s.sum_1 = take(g * 8);
+  s.sum_k = take(g * 8);
+  s.sum_a = take(g * 8);
   s.cand = take(c * kShort * 8);
+  s.cand2 = take(c * kShort * 8);
+  s.hist = take((size_t)rows * ((chunks + per - 1) / per) * kCutBins * 4);
   s.gmax = take(g * 4);
   s.smax = take(g * 16);
   s.low = take((size_t)rows * 4);
   s.count = take(c * 4);
+  s.count2 = take(c * 4);
+  s.cut = take((size_t)rows * 4);
   return s;
 }
 
@@ -1291,6 +1710,14 @@ int ffai_sample(const void* logits, int32_t logits_dtype, int32_t rows, int32_t 
   p.smax = reinterpret_cast<float*>(ws + sp.smax);
   p.low = reinterpret_cast<float*>(ws + sp.low);
   p.count = reinterpret_cast<int32_t*>(ws + sp.count);
+  p.sum_k = reinterpret_cast<double*>(ws + sp.sum_k);
+  p.sum_a = reinterpret_cast<double*>(ws + sp.sum_a);
+  p.cand2 = reinterpret_cast<uint64_t*>(ws + sp.cand2);
+  p.hist = reinterpret_cast<uint32_t*>(ws + sp.hist);
+  p.count2 = reinterpret_cast<int32_t*>(ws + sp.count2);
+  p.cut = reinterpret_cast<int32_t*>(ws + sp.cut);
+  p.per = sample_per(rows, p.chunks);
+  p.parts = (p.chunks + p.per - 1) / p.per;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool tiny = vocab < (logits_dtype == FFAI_F32 ? 4 : 8);  // less than a lane's load
   auto launch = [&](auto dt) {

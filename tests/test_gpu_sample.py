@@ -221,3 +221,59 @@ def test_short_workspace_is_refused(gpu):
     sample(l, u, workspace=torch.empty(n, dtype=torch.uint8, device=gpu))
     with pytest.raises(L.FfaiError, match="workspace"):
         sample(l, u, workspace=torch.empty(n - 1, dtype=torch.uint8, device=gpu))
+
+
+@pytest.mark.parametrize("vocab,rows", [(51865, 3), (131072, 2), (200001, 1), (300000, 2)])
+@pytest.mark.parametrize("kw", [dict(p=0.85), dict(p=0.999), dict(p=0.5, t=1.7), dict(mp=0.02),
+                                dict(p=0.9, mp=0.01), dict(p=0.9, mp=0.3, t=0.4), dict(p=1e-9),
+                                dict(p=-1.0), dict(p=0.6, t=math.inf)], ids=str)
+@pytest.mark.parametrize("sigma", [0.3, 3.0])
+def test_nuclei_and_minima_of_many_tokens(gpu, vocab, rows, kw, sigma):
+    """More tokens than a list holds, spread over several workgroups a row; logits of 16 bits, so
+    that many are equal, and (small sigma) more in the boundary's bins than are listed."""
+    for dtype in (torch.float32, torch.bfloat16):
+        l, u = make(gpu, rows, vocab, sigma=sigma, seed=vocab + rows, dtype=dtype)
+        check(l, u, **kw)
+
+
+def test_one_workspace_for_changing_settings(gpu):
+    """What a call leaves in the workspace is nothing to the next: rows that were wide nuclei are
+    settled by their list, greedy, unfiltered or minima in the next, and the other way round."""
+    rows, vocab = 6, 60000
+    l, u = make(gpu, rows, vocab, sigma=1.5, seed=8)
+    peaked = l.clone()
+    peaked[:, 7] = 30.0
+    masked = l.clone()
+    masked[1::2] = -math.inf
+    infinite = l.clone()
+    infinite[::2, 99] = math.inf
+    work = torch.empty(workspace_bytes(rows, vocab), dtype=torch.uint8, device=gpu)
+    work.fill_(255)
+    mixed = dict(t=torch.tensor([0.0, 1.0, 0.7, 1.0, 2.0, 1.0], device=gpu),
+                 k=torch.tensor([0, 40, 0, 0, 3000, 0], dtype=torch.int32, device=gpu),
+                 p=torch.tensor([0.9, 0.9, 0.8, 1.0, 0.9, 0.95], device=gpu),
+                 mp=torch.tensor([0.0, 0.0, 0.0, 0.01, 0.0, 0.001], device=gpu))
+    for x in (l, peaked, masked, infinite, l, infinite, peaked, l):
+        for kw in (dict(p=0.9), mixed, dict(mp=0.05), dict(), dict(k=30, p=0.9), dict(p=0.8, mp=0.01)):
+            got = sample(x, u, temperature=kw.get("t"), top_k=kw.get("k"), top_p=kw.get("p"),
+                         min_p=kw.get("mp"), workspace=work)
+            check(x, u, got=got, **kw)
+
+
+def test_wide_nuclei_in_a_graph(gpu):
+    rows, vocab = 5, 52000
+    l, u = make(gpu, rows, vocab, sigma=1.0, seed=21)
+    sample(l, u, top_p=0.9, min_p=0.001)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        tok, lp = sample(l, u, top_p=0.9, min_p=0.001)
+    for i in range(4):
+        a, b = make(gpu, rows, vocab, sigma=0.5 + i, seed=30 + i)
+        l.copy_(a)
+        u.copy_(b)
+        g.replay()
+        want = sample(l, u, top_p=0.9, min_p=0.001)
+        torch.cuda.synchronize()
+        assert torch.equal(tok, want[0]) and torch.equal(lp, want[1])
+        check(l, u, got=(tok, lp), p=0.9, mp=0.001)

@@ -1027,29 +1027,40 @@ __device__ __forceinline__ double row_weight(const SampleParams& p, int row, flo
   return wave_sum(w);
 }
 
-// A nucleus' histogram: bins of equal steps of the weight's logarithm below the maximum, weights as
-// integers of f32 exponentials whose sum over the row stays below 2^31 (adding them in any order
-// gives the same sum). They reach as far as the boundary may lie: n tokens of weight below
-// (1 - p) W / n weigh less than (1 - p) W together, and none below min_p is kept.
+// A nucleus' histogram: bins of equal steps of the weight's logarithm below the maximum. They reach
+// as far as the boundary may lie: n tokens of weight below (1 - p) W / n weigh less than (1 - p) W
+// together (and 2^8 further they do not matter to what follows the boundary either), and none below
+// min_p is kept. A bin's weights are integers of f32 exponentials (adding them in any order gives the
+// same sum), in a unit of the bin's own, 2^-unit 2^-`bits` of the largest: each is off by less than
+// `off` of itself, so that the sum over the bins up to one is known to that share of it, and what
+// follows it to that share of what follows.
 struct CutBins {
-  float m = 0.f, scale = 0.f, inv2f = 0.f;
-  int wshift = 0;
+  float m = 0.f, scale = 0.f, inv2f = 0.f, step = 0.f;
+  int bits = 0;
   CutBins() = default;
   __device__ __forceinline__ CutBins(float m, const RowSettings& s, int n, double whole) : m(m) {
-    double reach = s.mp > 0.0 ? -log2(s.mp) : log2((double)n / ((1.0 - (double)s.p) * whole));
-    reach = __builtin_fmin(__builtin_fmax(reach + 0.25, 1.0), 64.0);
+    double reach = s.mp > 0.0 ? 0.25 - log2(s.mp)
+                              : 8.25 + log2((double)n / ((1.0 - (double)s.p) * whole));
+    reach = __builtin_fmin(__builtin_fmax(reach, 1.0), 120.0);
     scale = fminf((float)(s.inv2 * (kCutBins / reach)), 1e30f);
     inv2f = fminf((float)s.inv2, 1e30f);
-    wshift = 30 - (int)__builtin_ceil(log2(fmax(whole, 1.0)));
+    step = (float)reach * (1.f / kCutBins);
+    bits = 31 - (32 - __builtin_clz((uint32_t)n));  // n times the largest stays below 2^32
   }
   // a bin where below kCutBins; it does not fall as logits do
   __device__ __forceinline__ float pos(float l) const {
     return l >= m ? 0.f : fminf((m - l) * scale, (float)kCutBins);
   }
-  __device__ __forceinline__ uint32_t value(float l) const {
-    const float wscale = __builtin_ldexpf(1.f, wshift);
-    return (uint32_t)(l >= m ? wscale : fast_exp2((l - m) * inv2f) * wscale);
+  __device__ __forceinline__ float unit(int b) const { return floorf((float)b * step); }
+  __device__ __forceinline__ uint32_t value(float l, int b) const {
+    const float y = l >= m ? 0.f : (l - m) * inv2f;
+    return (uint32_t)(fast_exp2(y + unit(b)) * __builtin_ldexpf(1.f, bits) + 0.5f);
   }
+  __device__ __forceinline__ double weight_of(uint32_t c, int b) const {
+    return __builtin_ldexp((double)c, -bits - (int)unit(b));
+  }
+  // (a value is 2^(bits - 1) units at least, rounded to one; an exponent is off by 2^-16)
+  __device__ __forceinline__ double off() const { return __builtin_ldexp(1.0, -bits) + 0x1p-15; }
 };
 
 // Sums over the groups of a chunk from those of the waves' loads: entry n covers elements
@@ -1145,7 +1156,7 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
           const float l = cur.v[e];
           if (nucleus) {
             const float at = bins.pos(l);
-            if (at < (float)kCutBins) atomicAdd(&hist[(int)at], bins.value(l));
+            if (at < (float)kCutBins) atomicAdd(&hist[(int)at], bins.value(l, (int)at));
           }
           if (minima) {
             if (__ballot(l >= m || (l - m) * inv2f >= min_y)) {
@@ -1347,21 +1358,28 @@ __global__ __launch_bounds__(kSpread) void sample_spread_kernel(SampleParams p) 
   double w[PB], sum = 0.0, total;
 #pragma unroll
   for (int e = 0; e < PB; ++e) {
-    w[e] = __builtin_ldexp((double)c[e], -bins.wshift);
+    w[e] = bins.weight_of(c[e], PB * tid + e);
     sum += w[e];
   }
   double run = block_scan(sh, sum, &total);
-  // (an integer weight is truncated: one step an element)
-  const double slack = total * 0x1p-17 + __builtin_ldexp((double)p.vocab, -bins.wshift);
+  const double off = bins.off(), eps = W * 1e-13, rest = (1.0 - (double)s.p) * W * 0x1p-8;
   int b0 = kCutBins, b1 = kCutBins;
 #pragma unroll
   for (int e = 0; e < PB; ++e) {
     run += w[e];
-    if (run >= want - slack) b0 = min(b0, PB * tid + e);
-    if (run >= want + slack) b1 = min(b1, PB * tid + e);
+    // the weight up to this bin's end: by what it is, or (all the row reached) by what follows
+    double least = run * (1.0 - off), most = run * (1.0 + off);
+    if (s.mp <= 0.0) {
+      const double after = total - run;
+      least = __builtin_fmax(least, W - after * (1.0 + off) - rest);
+      most = __builtin_fmin(most, W - after * (1.0 - off));
+    }
+    if (most + eps >= want) b0 = min(b0, PB * tid + e);
+    if (least - eps >= want) b1 = min(b1, PB * tid + e);
   }
   block_min_max(sh, 0, b0, -b1);
-  const int lo = sh.i[0], hi = -sh.i[1];
+  // (with min_p the bins reach past all of S1, which the boundary is in)
+  const int hi = min(-sh.i[1], s.mp > 0.0 ? kCutBins - 1 : kCutBins), lo = min(sh.i[0], hi);
   if (part == 0 && tid == 0) p.cut[row] = hi < kCutBins ? 1 : 0;
   if (hi >= kCutBins) return;
   // ---- the logits at the bins' ends, by bisection: the least key of bins [0, lo - 1] (lanes 0 ..

@@ -225,6 +225,8 @@ def test_short_workspace_is_refused(gpu):
 
 @pytest.mark.parametrize("vocab,rows", [(51865, 3), (131072, 2), (200001, 1), (300000, 2)])
 @pytest.mark.parametrize("kw", [dict(p=0.85), dict(p=0.999), dict(p=0.5, t=1.7), dict(mp=0.02),
+                                dict(p=0.99999, t=0.8), dict(p=1 - 2.0 ** -24, t=0.9),
+                                dict(p=0.99999, mp=0.001),
                                 dict(p=0.9, mp=0.01), dict(p=0.9, mp=0.3, t=0.4), dict(p=1e-9),
                                 dict(p=-1.0), dict(p=0.6, t=math.inf)], ids=str)
 @pytest.mark.parametrize("sigma", [0.3, 3.0])

@@ -131,11 +131,16 @@ struct PrefixPlan {
   size_t part_bytes, bytes;
 };
 
-// By capacity, which is what the host knows: five rounds of a workgroup's eight waves. 5 beams x 16
-// heads, 37 shared and 40 own keys of capacity 448: 5.8 us (7.05 in two launches), 8 x 5 beams x 16
-// heads, 224 shared and 200 own keys (24 tiles) with an f32 result 11.5 (13.2); head_dim 128, 8 x 16
-// slots x 32 heads, 128 and 128 keys 18.3 (23.1).
-constexpr int64_t kWholeTiles = 40;
+// Tiles (by capacity, which is what the host knows) up to which a workgroup of eight waves attends
+// whole slots: where such workgroups fill the GPU (one for most CUs, or tiles enough for pieces to
+// fill it anyway), pieces win nothing but shorter chains; where they do not, pieces win the other
+// CUs. Both ways, us (one slot a workgroup unless they exceed 256): head_dim
+// 64, 5 slots x 16 heads, 3, 9 and 17 tiles 5.2 (7.0), 7.2 (7.3) and 9.1 (7.4); 32 x 16, 17 and 33
+// tiles 10.2 (11.9) and 15.9 (16.2); head_dim 128, 5 x 16, 3 and 9 tiles 6.0 (7.3) and 9.7 (8.5);
+// 32 x 16, 9 and 17 tiles 13.1 (13.5) and 18.8 (18.6).
+constexpr int64_t whole_tiles(int64_t head_dim, bool full) {
+  return head_dim == 64 ? (full ? 40 : 9) : (full ? 17 : 6);
+}
 
 PrefixPlan plan_prefix(const ffai_kv_cache* pre, const ffai_kv_cache* own, int heads_q, int q_len) {
   PrefixPlan p{};
@@ -151,8 +156,15 @@ PrefixPlan plan_prefix(const ffai_kv_cache* pre, const ffai_kv_cache* own, int h
   // merge cost as much as the attention of a short step).
   if (p.R <= block) {
     const int64_t per = own->slots / pre->slots;
-    const int64_t bs = std::min<int64_t>(per, block / p.R);
-    if (tiles_p + bs * tiles_o <= kWholeTiles) {
+    // As few slots to a workgroup as keep one workgroup or less to a CU (110 slots x 8 heads, 48 shared
+    // and 5 own keys: 4 slots 8.4 us, 32 slots 18.2; 8 x 5 slots x 16 heads, 224 shared and 200 own
+    // keys: 3 slots 10.1, 5 slots 11.0).
+    const int64_t most = std::min<int64_t>(per, block / p.R);
+    int64_t bs = 1;
+    while (bs < most && units * ceil_div(per, bs) > 256) ++bs;
+    const bool full = units * ceil_div(per, bs) >= 192 ||
+                      units * tiles_p + own->slots * own->heads * tiles_o >= 8 * 256;
+    if (tiles_p + bs * tiles_o <= whole_tiles(own->head_dim, full)) {
       p.block_slots = (int)bs;
       p.blocks_p = (int)ceil_div(per, bs);
       p.pieces_p = 1;
@@ -299,7 +311,7 @@ int ffai_prefix_attn_fwd(const ffai_kv_cache* prefix, const ffai_kv_cache* own, 
   if (pl.block_slots > 0) {
     p.block_slots = pl.block_slots;
     if (parts != kPartsOne && p.R <= 16) {  // (the parts leave registers for 16 rows)
-      p.block_slots = std::min(p.per, 16 / p.R);
+      p.block_slots = std::min(p.block_slots, 16 / p.R);
       p.pre.row_blocks = (p.per + p.block_slots - 1) / p.block_slots;
     }
     const hipError_t e = dt == FFAI_F16

@@ -313,3 +313,32 @@ def test_a_short_workspace_is_refused(gpu):
     plan(x["q"], workspace=torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=gpu))
     with pytest.raises(L.FfaiError, match="workspace"):
         plan(x["q"], workspace=torch.empty(plan.workspace_bytes - 1, dtype=torch.uint8, device=gpu))
+
+
+# so many heads that a workgroup takes several slots: their rows side by side in one or two blocks
+# of 16 columns, each slot's own tiles masked for the others
+SIDE = {
+    "one row a slot": (2, 24, 32, 1, 1, 64, [70, 0], [i % 81 for i in range(48)], 70, 80),
+    "four rows, two blocks": (2, 24, 32, 4, 1, 64, [130, 3], [(7 * i) % 65 for i in range(48)], 130, 64),
+    "tokens": (1, 40, 64, 1, 2, 128, [65], [(3 * i) % 64 for i in range(40)], 65, 63),
+}
+
+
+@pytest.mark.parametrize("shape", SIDE, ids=[s.replace(" ", "_") for s in SIDE])
+@pytest.mark.parametrize("io", IO, ids=["-".join(i) for i in IO])
+def test_slots_side_by_side(gpu, shape, io):
+    q, kv, out = io
+    gr, per, hkv, rep, t, d, pl, ol, pc, oc = SIDE[shape]
+    x = make(gpu, gr, per, hkv, rep, t, d, pl, ol, pc, oc, q, kv, seed=31)
+    plan = PrefixAttention(*caches(x), hkv * rep, t, q_dtype=DT[q], out_dtype=DT[out], scale=d ** -0.5)
+    assert plan.workspace_bytes == 0 and plan.plan()["row_block"] > rep * t
+    got = plan(x["q"])
+    check(got, x, d ** -0.5, DT[out])
+    # two slots of non-finite values: the others' results are what they were
+    odd = torch.tensor([3, 22], device=gpu)
+    for name, value in (("ov", float("inf")), ("ok", float("nan")), ("ov", float("nan"))):
+        x[name][odd] = value
+        again = plan(x["q"])
+        keep = torch.ones(len(ol), dtype=torch.bool, device=gpu)
+        keep[odd] = False
+        assert torch.equal(again[keep], got[keep])

@@ -249,9 +249,9 @@ __device__ __forceinline__ int wave_max(int v) {
 }
 
 // ---- scan --------------------------------------------------------------------------------------
-template <int DT, bool TINY>
+template <int DT>
 __global__ __launch_bounds__(256) void sample_scan_kernel(SampleParams p) {
-  constexpr int EPL = Lane<DT, TINY>::EPL, IT = kGroup / (64 * EPL);
+  constexpr int EPL = Lane<DT, false>::EPL, IT = kGroup / (64 * EPL);
   const int row = wg_id_y(), lane = item_id() & 63;
   const int group = __builtin_amdgcn_readfirstlane(wg_id_x() * 4 + (item_id() >> 6));
   if (group >= p.groups) return;
@@ -260,9 +260,9 @@ __global__ __launch_bounds__(256) void sample_scan_kernel(SampleParams p) {
   const int end = min((group + 1) * kGroup, p.vocab);
   u32x4 raw[IT];
 #pragma unroll
-  for (int i = 0; i < IT; ++i) raw[i] = Lane<DT, TINY>::raw(x, base + i * 64 * EPL, p.vocab);
+  for (int i = 0; i < IT; ++i) raw[i] = Lane<DT, false>::raw(x, base + i * 64 * EPL, p.vocab);
   const RowSettings s = settings(p, row);
-  Lane<DT, TINY> a[IT];
+  Lane<DT, false> a[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i)
     a[i].take(raw[i], base + i * 64 * EPL, p.vocab, end, (group + 1) * kGroup);
@@ -285,9 +285,9 @@ __global__ __launch_bounds__(256) void sample_scan_kernel(SampleParams p) {
     // sixteen in line (the code of a launch comes cold from memory)
 #pragma unroll 1
     for (int i = 0; i < IT; ++i) {
-      Lane<DT, TINY> b;
+      Lane<DT, false> b;
       const int j = base + i * 64 * EPL;
-      b.take(Lane<DT, TINY>::raw(x, j, p.vocab), j, p.vocab, end, (group + 1) * kGroup);
+      b.take(Lane<DT, false>::raw(x, j, p.vocab), j, p.vocab, end, (group + 1) * kGroup);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) st += weight(b.v[e], m, s.inv2);
     }
@@ -1077,9 +1077,9 @@ __device__ __forceinline__ void put_group_sums(const SampleParams& p, double* to
   to[(int64_t)row * p.groups + g] = x;
 }
 
-template <int DT, bool TINY>
+template <int DT>
 __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
-  constexpr int EPL = Lane<DT, TINY>::EPL, IT = kChunk / (256 * EPL);
+  constexpr int EPL = Lane<DT, false>::EPL, IT = kChunk / (256 * EPL);
   constexpr int kHeld = 1024;  // maxima at most
   __shared__ float bound, top;
   __shared__ double whole;
@@ -1103,7 +1103,7 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
   u32x4 a[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i)
-    a[i] = Lane<DT, TINY>::raw(x, c0 * kChunk + (i * 256 + tid) * EPL, p.vocab);
+    a[i] = Lane<DT, false>::raw(x, c0 * kChunk + (i * 256 + tid) * EPL, p.vocab);
   if (tid < 2) count[tid] = 0;
   if (nucleus)
     for (int b = tid; b < kCutBins; b += 256) hist[b] = 0;
@@ -1147,8 +1147,8 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
 #pragma unroll 1
       for (int i = 0; i < IT; ++i) {
         const int i0 = c * kChunk + (i * 256 + tid) * EPL;
-        Lane<DT, TINY> cur;
-        cur.take(Lane<DT, TINY>::raw(x, i0, p.vocab), i0, p.vocab, p.vocab,
+        Lane<DT, false> cur;
+        cur.take(Lane<DT, false>::raw(x, i0, p.vocab), i0, p.vocab, p.vocab,
                  c * kChunk + (i + 1) * 256 * EPL);
         double sum = 0.0;
 #pragma unroll
@@ -1174,7 +1174,7 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int i0 = c * kChunk + (i * 256 + tid) * EPL;
-      Lane<DT, TINY> cur;
+      Lane<DT, false> cur;
       cur.take(a[i], i0, p.vocab, p.vocab, c * kChunk + (i + 1) * 256 * EPL);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
@@ -1188,7 +1188,7 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
         if (take && at < kShort) to[at] = rank_of(l, i0 + e);
       }
       // the next chunk's loads go out as this one's are done with
-      a[i] = Lane<DT, TINY>::raw(x, i0 + kChunk, p.vocab);
+      a[i] = Lane<DT, false>::raw(x, i0 + kChunk, p.vocab);
     }
     __syncthreads();
     // (the next chunk uses the other word and row, and its barrier comes before these ones' reuse)
@@ -1314,12 +1314,61 @@ __device__ __forceinline__ bool settled(const SampleParams& p, SH& sh, int row, 
   return x * (1.0 - 1e-12) >= (double)s.p * W;
 }
 
+// The logits [*bottom, *top] of the bins that the boundary may lie in, by as much as the histogram may be
+// off; c: the bins PB t .. of thread t. False where the bins do not reach it.
+template <int PB, class SH>
+__device__ __forceinline__ bool cut_range(SH& sh, const CutBins& bins, const RowSettings& s,
+                                          const uint32_t (&c)[PB], double W, double want, float* top,
+                                          float* bottom) {
+  const int tid = item_id(), lane = tid & 63;
+  double w[PB], sum = 0.0, total;
+#pragma unroll
+  for (int e = 0; e < PB; ++e) {
+    w[e] = bins.weight_of(c[e], PB * tid + e);
+    sum += w[e];
+  }
+  double run = block_scan(sh, sum, &total);
+  const double off = bins.off(), eps = W * 1e-13, rest = (1.0 - (double)s.p) * W * 0x1p-8;
+  int b0 = kCutBins, b1 = kCutBins;
+#pragma unroll
+  for (int e = 0; e < PB; ++e) {
+    run += w[e];
+    // the weight up to this bin's end: by what it is, or (all the row reached) by what follows
+    double least = run * (1.0 - off), most = run * (1.0 + off);
+    if (s.mp <= 0.0) {
+      const double after = total - run;
+      least = __builtin_fmax(least, W - after * (1.0 + off) - rest);
+      most = __builtin_fmin(most, W - after * (1.0 - off));
+    }
+    if (most + eps >= want) b0 = min(b0, PB * tid + e);
+    if (least - eps >= want) b1 = min(b1, PB * tid + e);
+  }
+  block_min_max(sh, 0, b0, -b1);
+  // (with min_p the bins reach past all of S1, which the boundary is in)
+  const int hi = min(-sh.i[1], s.mp > 0.0 ? kCutBins - 1 : kCutBins), lo = min(sh.i[0], hi);
+  if (hi >= kCutBins) return false;
+  // the bins' ends by bisection: the least key of bins [0, lo - 1] (lanes 0 .. 31) and of [0, hi]
+  uint32_t kx = key_of(kNegInf) + 1, ky = key_of(bins.m);
+  const float b = (float)(lane < 32 ? lo : hi + 1);
+  while (__ballot(kx < ky)) {
+    const uint32_t mid = kx + (ky - kx) / 2;
+    if (kx < ky) {
+      if (bins.pos(of_key(mid)) < b) ky = mid;
+      else kx = mid + 1;
+    }
+  }
+  const uint32_t k_lo = (uint32_t)__shfl((int)kx, 0), k_hi = (uint32_t)__shfl((int)kx, 32);
+  *top = lo == 0 ? bins.m : of_key(k_lo - 1);
+  *bottom = of_key(k_hi);
+  return true;
+}
+
 // An open nucleus, spread over the row's chunks: the bins of the histogram that the limit may lie
 // in, by as much as its integers may be off; the tokens in them are listed, the weights above them
 // summed by group; the pick finishes the row.
-template <int DT, bool TINY>
+template <int DT>
 __global__ __launch_bounds__(kSpread) void sample_spread_kernel(SampleParams p) {
-  constexpr int EPL = Lane<DT, TINY>::EPL, IT = kChunk / (kSpread * EPL);
+  constexpr int EPL = Lane<DT, false>::EPL, IT = kChunk / (kSpread * EPL);
   __shared__ SpreadShared sh;
   const int part = wg_id_x(), row = wg_id_y();
   const int tid = item_id(), lane = tid & 63;
@@ -1355,48 +1404,11 @@ __global__ __launch_bounds__(kSpread) void sample_spread_kernel(SampleParams p) 
 #pragma unroll 4
     for (int j = 0; j < p.parts; ++j) c += h[(int64_t)j * (kCutBins / 4)];
   }
-  double w[PB], sum = 0.0, total;
-#pragma unroll
-  for (int e = 0; e < PB; ++e) {
-    w[e] = bins.weight_of(c[e], PB * tid + e);
-    sum += w[e];
-  }
-  double run = block_scan(sh, sum, &total);
-  const double off = bins.off(), eps = W * 1e-13, rest = (1.0 - (double)s.p) * W * 0x1p-8;
-  int b0 = kCutBins, b1 = kCutBins;
-#pragma unroll
-  for (int e = 0; e < PB; ++e) {
-    run += w[e];
-    // the weight up to this bin's end: by what it is, or (all the row reached) by what follows
-    double least = run * (1.0 - off), most = run * (1.0 + off);
-    if (s.mp <= 0.0) {
-      const double after = total - run;
-      least = __builtin_fmax(least, W - after * (1.0 + off) - rest);
-      most = __builtin_fmin(most, W - after * (1.0 - off));
-    }
-    if (most + eps >= want) b0 = min(b0, PB * tid + e);
-    if (least - eps >= want) b1 = min(b1, PB * tid + e);
-  }
-  block_min_max(sh, 0, b0, -b1);
-  // (with min_p the bins reach past all of S1, which the boundary is in)
-  const int hi = min(-sh.i[1], s.mp > 0.0 ? kCutBins - 1 : kCutBins), lo = min(sh.i[0], hi);
-  if (part == 0 && tid == 0) p.cut[row] = hi < kCutBins ? 1 : 0;
-  if (hi >= kCutBins) return;
-  // ---- the logits at the bins' ends, by bisection: the least key of bins [0, lo - 1] (lanes 0 ..
-  // 31) and of bins [0, hi]
-  uint32_t kx = key_of(kNegInf) + 1, ky = key_of(m);
-  {
-    const float b = (float)(lane < 32 ? lo : hi + 1);
-    while (__ballot(kx < ky)) {
-      const uint32_t mid = kx + (ky - kx) / 2;
-      if (kx < ky) {
-        if (bins.pos(of_key(mid)) < b) ky = mid;
-        else kx = mid + 1;
-      }
-    }
-  }
-  const uint32_t k_lo = (uint32_t)__shfl((int)kx, 0), k_hi = (uint32_t)__shfl((int)kx, 32);
-  const float ftop = lo == 0 ? m : of_key(k_lo - 1), fbottom = of_key(k_hi);
+  uint32_t cb[PB] = {c[0], c[1], c[2], c[3]};
+  float ftop, fbottom;
+  const bool cut = cut_range<PB>(sh, bins, s, cb, W, want, &ftop, &fbottom);
+  if (part == 0 && tid == 0) p.cut[row] = cut ? 1 : 0;
+  if (!cut) return;
   // ---- list what the bins hold, sum what lies above them
   const store_t<DT>* x = reinterpret_cast<const store_t<DT>*>(p.logits) + (int64_t)row * p.ls;
   const int c0 = part * p.per, c1 = min(c0 + p.per, p.chunks);
@@ -1404,7 +1416,7 @@ __global__ __launch_bounds__(kSpread) void sample_spread_kernel(SampleParams p) 
   u32x4 r[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i)
-    r[i] = Lane<DT, TINY>::raw(x, c0 * kChunk + (i * kSpread + tid) * EPL, p.vocab);
+    r[i] = Lane<DT, false>::raw(x, c0 * kChunk + (i * kSpread + tid) * EPL, p.vocab);
   if (tid < 2) count[tid] = 0;
   __syncthreads();
 #pragma unroll 1
@@ -1415,7 +1427,7 @@ __global__ __launch_bounds__(kSpread) void sample_spread_kernel(SampleParams p) 
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int i0 = ch * kChunk + (i * kSpread + tid) * EPL;
-      Lane<DT, TINY> cur;
+      Lane<DT, false> cur;
       cur.take(r[i], i0, p.vocab, p.vocab, ch * kChunk + (i + 1) * kSpread * EPL);
       double above = 0.0;
 #pragma unroll
@@ -1431,7 +1443,7 @@ __global__ __launch_bounds__(kSpread) void sample_spread_kernel(SampleParams p) 
         }
         if (__ballot(l > ftop)) above += l > ftop ? weight(l, m, s.inv2) : 0.0;
       }
-      r[i] = Lane<DT, TINY>::raw(x, i0 + kChunk, p.vocab);
+      r[i] = Lane<DT, false>::raw(x, i0 + kChunk, p.vocab);
       above = wave_sum(above);
       if (lane == 0) rd[i * SpreadShared::NW + wave] = above;
     }
@@ -1445,26 +1457,11 @@ __global__ __launch_bounds__(kSpread) void sample_spread_kernel(SampleParams p) 
   }
 }
 
-// A nucleus whose boundary's bins are listed (n tokens, sh.raw): ordered, the definition applied;
-// then the token by the groups' weights.
-template <int DT, bool TINY>
-__device__ __forceinline__ int finish_cut(const SampleParams& p, const Row<DT, TINY>& row,
-                                          PickShared& sh, int rowi, int n, const RowSettings& s,
-                                          float m, double W, double u) {
-  const int tid = item_id(), lane = tid & 63;
-  const int64_t at = (int64_t)rowi * p.groups;
-  double above = 0.0, w1 = W;
-  if (s.mp > 0.0) w1 = 0.0;
-#pragma unroll 1
-  for (int g = lane; g < p.groups; g += 64) {
-    above += p.sum_a[at + g];
-    if (s.mp > 0.0) w1 += p.sum_k[at + g];
-  }
-  above = wave_sum(above);
-  if (s.mp > 0.0) w1 = wave_sum(w1);
-  const double want = (double)s.p * w1;
-  for (int j = tid; j < n; j += kPick) sh.sorted[j] = sh.raw[j];
-  __syncthreads();
+// The list sh.sorted[0 .. n) of a nucleus' bins, ordered; the place of the last kept token in it. above:
+// the weight of what comes before the list.
+__device__ __forceinline__ int cut_list(PickShared& sh, int n, const RowSettings& s, float m,
+                                        double above, double want) {
+  const int tid = item_id();
   sort_list(sh.sorted, n);
   constexpr int PL = kList / kPick;
   double w[PL], mine = 0.0, total;
@@ -1481,7 +1478,30 @@ __device__ __forceinline__ int finish_cut(const SampleParams& p, const Row<DT, T
     before += w[e];
   }
   block_min_max(sh, 0, 0, last);
-  last = sh.i[1];
+  return sh.i[1];
+}
+
+// A nucleus whose boundary's bins are listed (n tokens, sh.raw): ordered, the definition applied;
+// then the token by the groups' weights.
+template <int DT>
+__device__ __forceinline__ int finish_cut(const SampleParams& p, const Row<DT, false>& row,
+                                          PickShared& sh, int rowi, int n, const RowSettings& s,
+                                          float m, double W, double u) {
+  const int tid = item_id(), lane = tid & 63;
+  const int64_t at = (int64_t)rowi * p.groups;
+  double above = 0.0, w1 = W;
+  if (s.mp > 0.0) w1 = 0.0;
+#pragma unroll 1
+  for (int g = lane; g < p.groups; g += 64) {
+    above += p.sum_a[at + g];
+    if (s.mp > 0.0) w1 += p.sum_k[at + g];
+  }
+  above = wave_sum(above);
+  if (s.mp > 0.0) w1 = wave_sum(w1);
+  const double want = (double)s.p * w1;
+  for (int j = tid; j < n; j += kPick) sh.sorted[j] = sh.raw[j];
+  __syncthreads();
+  const int last = cut_list(sh, n, s, m, above, want);
   const uint64_t low = sh.sorted[last];
   // the listed tokens that are kept join their groups, as multiples of 2^-52 of the largest weight
   // (adding integers in any order gives the same sum)
@@ -1489,11 +1509,13 @@ __device__ __forceinline__ int finish_cut(const SampleParams& p, const Row<DT, T
   for (int g = tid; g < p.groups; g += kPick) sums[g] = 0;
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < PL; ++e) {
-    const int j = PL * tid + e;
-    if (j <= last)
-      atomicAdd(reinterpret_cast<unsigned long long*>(&sums[index_of(sh.sorted[j]) / kGroup]),
-                (unsigned long long)(w[e] * 0x1p52));
+  for (int e = 0; e < kList / kPick; ++e) {
+    const int j = kList / kPick * tid + e;
+    if (j <= last) {
+      const uint64_t r = sh.sorted[j];
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sums[index_of(r) / kGroup]),
+                (unsigned long long)(weight(logit_of(r), m, s.inv2) * 0x1p52));
+    }
   }
   __syncthreads();
   return draw_groups<DT>(
@@ -1503,14 +1525,14 @@ __device__ __forceinline__ int finish_cut(const SampleParams& p, const Row<DT, T
 static_assert(sizeof(PickShared::ring) >= kMaxVocab / kGroup * sizeof(double), "a sum per group");
 
 // FILTER: rows may filter. (Without, a kernel of a tenth of the code, which comes cold from memory.)
-template <int DT, bool TINY, bool FILTER>
+template <int DT, bool FILTER>
 __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) char pick_lds[];
   using SH = std::conditional_t<FILTER, PickShared, DrawShared>;
   SH& sh = *reinterpret_cast<SH*>(pick_lds);
   const int rowi = wg_id_x(), tid = item_id(), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  Row<DT, TINY> row;
+  Row<DT, false> row;
   row.x = reinterpret_cast<const store_t<DT>*>(p.logits) + (int64_t)rowi * p.ls;
   row.n = p.vocab;
   if constexpr (FILTER) row.ring = sh.ring;
@@ -1554,12 +1576,12 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     for (int g = lane; g < p.groups; g += 64)
       if (gm[g] == m) g0 = min(g0, g);
     g0 = wave_min(g0);
-    constexpr int EPL = Row<DT, TINY>::EPL;
+    constexpr int EPL = Row<DT, false>::EPL;
     int f = 0x7fffffff;
 #pragma unroll 1
     for (int i = g0 * kGroup + (kGroup / 64 - EPL) + kGroup / 64 * lane; i >= g0 * kGroup + kGroup / 64 * lane; i -= EPL) {
-      Lane<DT, TINY> a;
-      a.take(Lane<DT, TINY>::raw(row.x, i, row.n), i, row.n, row.n, (g0 + 1) * kGroup);
+      Lane<DT, false> a;
+      a.take(Lane<DT, false>::raw(row.x, i, row.n), i, row.n, row.n, (g0 + 1) * kGroup);
 #pragma unroll
       for (int e = EPL - 1; e >= 0; --e)
         if (a.v[e] == m) f = i + e;
@@ -1609,30 +1631,241 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
   }
 }
 
+// ---- small vocabularies ------------------------------------------------------------------------
+// A row in the registers of one workgroup, 8 logits a thread: one launch. top_k: the k-th largest of
+// the threads' maxima bounds the list, as in the gather; a nucleus: its histogram in LDS, then the
+// boundary's bins listed.
+constexpr int kSmall = 8 * kPick;
+static_assert(sizeof(PickShared::bin) >= kCutBins * 4 && sizeof(PickShared::bin) >= kPick * 4, "");
+
 template <int DT, bool TINY>
+__global__ __launch_bounds__(kPick) void sample_small_kernel(SampleParams p) {
+  extern __shared__ __attribute__((aligned(16))) char pick_lds[];
+  PickShared& sh = *reinterpret_cast<PickShared*>(pick_lds);
+  constexpr int PER = 8, EPL = Lane<DT, TINY>::EPL;
+  const int rowi = wg_id_x(), tid = item_id(), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Row<DT, TINY> row;
+  row.x = reinterpret_cast<const store_t<DT>*>(p.logits) + (int64_t)rowi * p.ls;
+  row.n = p.vocab;
+  row.ring = sh.ring;
+  const int i0 = PER * tid;
+  u32x4 raw[PER / EPL];
+#pragma unroll
+  for (int j = 0; j < PER / EPL; ++j) raw[j] = Lane<DT, TINY>::raw(row.x, i0 + j * EPL, p.vocab);
+  const RowSettings s = settings(p, rowi);
+  const float uf = p.u[rowi];
+  const double u = is_nan(uf) || uf < 0.f ? 0.0 : (double)fminf(uf, 0x1.fffffep-1f);
+  float v[PER];
+  float mine = kNegInf;
+#pragma unroll
+  for (int j = 0; j < PER / EPL; ++j) {
+    Lane<DT, TINY> a;
+    a.take(raw[j], i0 + j * EPL, p.vocab, p.vocab, (wave + 1) * 64 * PER);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      v[j * EPL + e] = a.v[e];
+      mine = fmaxf(mine, a.v[e]);
+    }
+  }
+  {
+    const float x = wave_max_all(mine);
+    if (lane == 0) sh.red[wave] = x;
+    __syncthreads();
+  }
+  float m = kNegInf;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, (float)sh.red[w]);
+  if (m == kNegInf) {  // nothing to choose from (uniform)
+    if (tid == 0) {
+      p.tok[rowi] = -1;
+      if (p.lp) p.lp[rowi] = kNegInf;
+    }
+    return;
+  }
+  double logz = 0.0;
+  if (p.lp) {  // f32 exponentials, as in the scan
+    float x = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      x += fast_exp2((v[e] >= m ? 0.f : v[e] - m) * 1.44269504088896340736f);
+    logz = block_sum(sh, (double)x);
+  }
+  int token = -1;
+  uint64_t low = 0;  // kept: ranks from here up, of weight >= min_p
+  if (s.greedy) {
+    int f = 0x7fffffff;
+#pragma unroll
+    for (int e = PER - 1; e >= 0; --e)
+      if (v[e] == m) f = i0 + e;
+    block_min_max(sh, 0, f, 0);
+    token = sh.i[0];
+  } else {
+    if (s.k > 0) {
+      // ---- a list of the first k (sh.n: how many are listed)
+      float* top = reinterpret_cast<float*>(sh.bin);
+      top[tid] = mine;
+      if (tid == 0) sh.n = 0;
+      __syncthreads();
+      const int n_top = (p.vocab + PER - 1) / PER;
+      if (wave == 0) {
+        const float b = s.k <= n_top ? list_bound<kPick / 64>(top, n_top, s.k) : kNegInf;
+        if (lane == 0) sh.logz = (double)b;
+      }
+      __syncthreads();
+      const float bound = (float)sh.logz;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) append(sh, v[e] >= bound && v[e] > kNegInf, v[e], i0 + e);
+      __syncthreads();
+      const int n = sh.n;
+      if (n <= kShort) {
+        token = pick_short(sh, n, s, m, -1.0, u);
+      } else if (n <= kList) {
+        for (int j = tid; j < n; j += kPick) sh.sorted[j] = sh.raw[j];
+        __syncthreads();
+        sort_list(sh.sorted, n);
+        constexpr int PL = kList / kPick;
+        double w[PL], sum = 0.0, total;
+        bool in1[PL];
+#pragma unroll
+        for (int e = 0; e < PL; ++e) {
+          const int j = PL * tid + e;
+          w[e] = j < min(n, s.k) ? weight(logit_of(sh.sorted[j]), m, s.inv2) : 0.0;
+          in1[e] = j < min(n, s.k) && w[e] >= s.mp;
+          if (!in1[e]) w[e] = 0.0;
+          sum += w[e];
+        }
+        double run = block_scan(sh, sum, &total);
+        const double limit = (double)s.p * total;
+        int last = 0;
+#pragma unroll
+        for (int e = 0; e < PL; ++e) {
+          if (in1[e] && (s.p >= 1.f || run < limit)) last = PL * tid + e;
+          run += w[e];
+        }
+        block_min_max(sh, 0, 0, last);
+        low = sh.sorted[sh.i[1]];
+      } else {
+        token = pick_wide(row, sh, s, m, 0.0, u);
+      }
+    } else if (s.p < 1.f) {
+      double x = 0.0, y = 0.0, total;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const double w = weight(v[e], m, s.inv2);
+        x += w;
+        y += w >= s.mp ? w : 0.0;
+      }
+      const double W = block_sum(sh, x), w1 = s.mp > 0.0 ? block_sum(sh, y) : W;
+      const double want = (double)s.p * w1;
+      bool cut = m != __builtin_inff();
+      if (cut) {  // uniform
+        for (int b = tid; b < kCutBins; b += kPick) sh.bin[b] = 0;
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        const CutBins bins(m, s, p.vocab, W);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const float at = bins.pos(v[e]);
+          if (at < (float)kCutBins) atomicAdd(&sh.bin[(int)at], bins.value(v[e], (int)at));
+        }
+        __syncthreads();
+        constexpr int PB = kCutBins / kPick;
+        uint32_t c[PB];
+#pragma unroll
+        for (int e = 0; e < PB; ++e) c[e] = sh.bin[PB * tid + e];
+        float ftop, fbottom;
+        cut = cut_range<PB>(sh, bins, s, c, W, want, &ftop, &fbottom);
+        if (cut) {
+          x = 0.0;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) {
+            append(sh, v[e] >= fbottom && v[e] <= ftop, v[e], i0 + e);
+            if (__ballot(v[e] > ftop)) x += v[e] > ftop ? weight(v[e], m, s.inv2) : 0.0;
+          }
+          const double above = block_sum(sh, x);
+          const int n = sh.n;
+          cut = n > 0 && n <= kList;
+          if (cut) {
+            for (int j = tid; j < n; j += kPick) sh.sorted[j] = sh.raw[j];
+            __syncthreads();
+            low = sh.sorted[cut_list(sh, n, s, m, above, want)];
+          }
+        }
+      }
+      if (!cut) token = pick_wide(row, sh, s, m, W, u);
+    }
+    if (token < 0) {
+      // ---- the kept weights in index order
+      double w[PER], sum = 0.0, total;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        w[e] = rank_of(v[e], i0 + e) >= low ? weight(v[e], m, s.inv2) : 0.0;
+        if (!(w[e] >= s.mp)) w[e] = 0.0;
+        sum += w[e];
+      }
+      double run = block_scan(sh, sum, &total);
+      const double target = u * total;
+      int hit = 0x7fffffff, last = 0;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        if (w[e] > 0.0) {
+          last = i0 + e;
+          if (run + w[e] > target) hit = min(hit, last);
+        }
+        run += w[e];
+      }
+      block_min_max(sh, 0, hit, last);
+      token = sh.i[0] != 0x7fffffff ? sh.i[0] : sh.i[1];
+    }
+  }
+  if (tid == 0) {
+    p.tok[rowi] = token;
+    if (p.lp) {
+      const float l = load1<DT>(row.x, token);
+      const double d = l >= m ? 0.0 : (double)l - (double)m;
+      p.lp[rowi] = (float)(d - log(logz));
+    }
+  }
+}
+
+template <class K>
+hipError_t large_lds(K kernel) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PickShared));
+}
+
+// (TINY: fewer tokens than a lane's load)
+template <int DT, bool TINY>
+hipError_t launch_small(const SampleParams& p, hipStream_t st) {
+  static const hipError_t once = large_lds(sample_small_kernel<DT, TINY>);
+  if (once != hipSuccess) return once;
+  hipLaunchKernelGGL((sample_small_kernel<DT, TINY>), dim3((unsigned)p.rows), dim3(kPick),
+                     sizeof(PickShared), st, p);
+  return hipGetLastError();
+}
+
+template <int DT>
 hipError_t launch_sample(const SampleParams& p, hipStream_t st) {
-  static const hipError_t once = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(sample_pick_kernel<DT, TINY, true>),
-      hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PickShared));
+  if (p.vocab < Lane<DT, false>::EPL) return launch_small<DT, true>(p, st);
+  if (p.vocab <= kSmall) return launch_small<DT, false>(p, st);
+  static const hipError_t once = large_lds(sample_pick_kernel<DT, true>);
   if (once != hipSuccess) return once;
   const unsigned rows = (unsigned)p.rows;
   // what rows may do, as far as the host knows
   const bool counts = p.k || p.k_all > 0, nuclei = p.p || p.p_all < 1.f;
   const bool minima = p.mp || p.mp_all > 0.f, all_count = !p.k && p.k_all > 0 && p.k_all < p.vocab;
-  hipLaunchKernelGGL((sample_scan_kernel<DT, TINY>), dim3((unsigned)((p.groups + 3) / 4), rows),
-                     dim3(256), 0, st, p);
+  hipLaunchKernelGGL(sample_scan_kernel<DT>, dim3((unsigned)((p.groups + 3) / 4), rows), dim3(256), 0,
+                     st, p);
   if (!counts && !nuclei && !minima) {
-    hipLaunchKernelGGL((sample_pick_kernel<DT, TINY, false>), dim3(rows), dim3(kPick),
-                       sizeof(DrawShared), st, p);
+    hipLaunchKernelGGL((sample_pick_kernel<DT, false>), dim3(rows), dim3(kPick), sizeof(DrawShared), st,
+                       p);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((sample_gather_kernel<DT, TINY>), dim3((unsigned)p.parts, rows), dim3(256), 0, st,
-                     p);
+  hipLaunchKernelGGL(sample_gather_kernel<DT>, dim3((unsigned)p.parts, rows), dim3(256), 0, st, p);
   if (nuclei && !all_count)
-    hipLaunchKernelGGL((sample_spread_kernel<DT, TINY>), dim3((unsigned)p.parts, rows), dim3(kSpread),
-                       0, st, p);
-  hipLaunchKernelGGL((sample_pick_kernel<DT, TINY, true>), dim3(rows), dim3(kPick), sizeof(PickShared),
-                     st, p);
+    hipLaunchKernelGGL(sample_spread_kernel<DT>, dim3((unsigned)p.parts, rows), dim3(kSpread), 0, st, p);
+  hipLaunchKernelGGL((sample_pick_kernel<DT, true>), dim3(rows), dim3(kPick), sizeof(PickShared), st, p);
   return hipGetLastError();
 }
 
@@ -1746,14 +1979,9 @@ int ffai_sample(const void* logits, int32_t logits_dtype, int32_t rows, int32_t 
   p.per = sample_per(rows, p.chunks);
   p.parts = (p.chunks + p.per - 1) / p.per;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool tiny = vocab < (logits_dtype == FFAI_F32 ? 4 : 8);  // less than a lane's load
-  auto launch = [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    return tiny ? launch_sample<DT, true>(p, st) : launch_sample<DT, false>(p, st);
-  };
-  const hipError_t e = logits_dtype == FFAI_F32   ? launch(std::integral_constant<int, kF32>{})
-                       : logits_dtype == FFAI_F16 ? launch(std::integral_constant<int, kF16>{})
-                                                  : launch(std::integral_constant<int, kBF16>{});
+  const hipError_t e = logits_dtype == FFAI_F32   ? launch_sample<kF32>(p, st)
+                       : logits_dtype == FFAI_F16 ? launch_sample<kF16>(p, st)
+                                                  : launch_sample<kBF16>(p, st);
   if (e != hipSuccess) return api_fail(FFAI_ERR_HIP, hipGetErrorString(e));
   return FFAI_OK;
 }

@@ -1,8 +1,10 @@
 // Sampling of one token per row of logits (include/ffai_sample.h).
 //
-// Two launches, three where a row may filter, four where it may by weight:
+// One launch for small vocabularies; else two, three where a row may filter, four where it may by
+// weight:
+//   * sample_small_kernel, up to 8192 tokens (16384 with filters): all of it, a row in registers;
 //   * sample_scan_kernel reads the logits, spread over the whole GPU: of every 1024 elements (a
-//     wave's) the maximum, those of its four rows of lanes, and the weights' sum;
+//     wave's) the maximum, those of its quads of lanes, and the weights' sum;
 //   * sample_gather_kernel: nearly always few tokens can be kept. The k-th largest group maximum
 //     bounds the k-th largest logit from below, so a second spread pass lists everything from there
 //     up (k and a few tokens more). Beside that, where there is no k: min_p's kept weight of each
@@ -23,7 +25,8 @@
 //
 // Few rows are bound by the launches and their chains of loads: 5 x 51865 f32 at a temperature
 // 12 us, 64 x 51865 with top-k and top-p 26, one row of 51865 top-k 18, top-p over thousands of
-// tokens 45 (81 with the histograms in the picking workgroup alone). Many rows by instructions: 256 x
+// tokens 45 (81 with the histograms in the picking workgroup alone); 12 x 1906 top-k in one launch 17
+// (56 in three), 26 x 1182 top-p 25 (44 in four). Many rows by instructions: 256 x
 // 131072 bf16, settings of each row's own, 126 us (235): the scan 32, the gather 36, the nuclei's
 // spread 32, the pick 27. The spread costs rows that need none 2 to 3 us.
 #include "../../include/ffai_sample.h"
@@ -47,6 +50,7 @@ constexpr int kBins = 4096;
 constexpr int kChunk = 4096;  // elements of a gather workgroup's share
 constexpr int kParts = 16;    // gather workgroups of a row, about
 constexpr int kCutBins = 2048;  // bins of a nucleus' histogram
+constexpr int kHeld = 1024;   // maxima that bound a list, at most
 constexpr int kAhead = 4;     // steps of a pass over a row that a wave loads ahead
 
 struct SampleParams {
@@ -65,7 +69,7 @@ struct SampleParams {
   double* sum_t;   // [row][group] sum of exp((l - group max) / T)
   double* sum_1;   // [row][group] sum of exp(l - group max)
   float* gmax;     // [row][group] maxima
-  float* smax;     // [row][group][4] of the group's four rows of lanes
+  float* smax;     // [row][group][16] of the group's quads of lanes
   float* low;      // [row] the least logit that is listed; -inf: no list
   int32_t* count;  // [row][chunk] listed tokens (kShort at most are held)
   uint64_t* cand;  // [row][chunk][kShort] their ranks, in no order
@@ -273,9 +277,9 @@ __global__ __launch_bounds__(256) void sample_scan_kernel(SampleParams p) {
     for (int e = 0; e < EPL; ++e) m = fmaxf(m, a[i].v[e]);
   m = fmaxf(m, dpp_mov<0xb1>(m));   // quad_perm [1,0,3,2]
   m = fmaxf(m, dpp_mov<0x4e>(m));   // quad_perm [2,3,0,1]
+  if ((lane & 3) == 0) p.smax[((int64_t)row * p.groups + group) * 16 + (lane >> 2)] = m;
   m = fmaxf(m, dpp_mov<0x124>(m));  // row_ror:4
   m = fmaxf(m, dpp_mov<0x128>(m));  // row_ror:8: the row's maximum in each of its 16 lanes
-  if ((lane & 15) == 0) p.smax[((int64_t)row * p.groups + group) * 4 + (lane >> 4)] = m;
   m = quad_max(m);
   // the weights' sum is needed unless top-k lists the kept tokens anyway (or the row is greedy)
   const bool need_t = !s.greedy && s.k == 0;
@@ -959,35 +963,34 @@ __device__ __forceinline__ int pick_wide(const Row<DT, TINY>& row, PickShared& s
 }
 
 // ---- gather ------------------------------------------------------------------------------------
-// Which maxima bound a row's list: the `k`-th largest of `n` (`fine`: of the quarter groups), n 0
-// for no list. k is top_k, or for nuclei and minima a guess at what they leave.
+// Which maxima bound a row's list: the `k`-th largest of `n`, of a group or a quarter or a sixteenth
+// of one each (`span` of the sixteenths); n 0 for no list. k is top_k, or for nuclei and minima a
+// guess at what they leave.
 struct ListRule {
-  int k, n;
-  bool fine;
+  int k, n, span;
 };
 __device__ __forceinline__ ListRule list_rule(const RowSettings& s, int groups) {
   ListRule r;
   r.k = s.k > 0 ? s.k : 96;
   // (with k near the number of maxima the bound falls far below the k-th logit)
-  r.fine = 4 * r.k > 3 * groups;
-  r.n = r.fine ? 4 * groups : groups;
-  if (s.k == 0) r.k = min(r.k, max(1, r.n * 3 / 4));
-  if (r.k > r.n || r.k > kShort) r.n = 0;
+  r.span = 4 * r.k <= 3 * groups ? 16 : r.k <= 3 * groups || groups > kHeld / 16 ? 4 : 1;
+  r.n = groups * (16 / r.span);
+  if (r.k > r.n || r.k > kShort || r.n > kHeld) r.n = 0;
   return r;
 }
 
 // A bound that the k-th largest of n maxima does not fall below, one wave: bisection of the keys'
 // range, the maxima in registers (PER a lane). 20 steps leave a millionth of the range, which costs a
 // few tokens more on the list. -inf where fewer than k are finite.
-template <int PER>
-__device__ __forceinline__ float list_bound(const float* gm, int n, int k) {
+template <int PER, class F>
+__device__ __forceinline__ float list_bound(F maximum, int n, int k) {
   const int lane = item_id() & 63;
   const uint32_t none = key_of(kNegInf);
   uint32_t key[PER], hi = none, least = 0xffffffffu;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int g = 64 * j + lane;
-    key[j] = g < n ? key_of(gm[g]) : none;
+    key[j] = g < n ? key_of(maximum(g)) : none;
     hi = max(hi, key[j]);
     least = min(least, key[j] > none ? key[j] : 0xffffffffu);
   }
@@ -1080,7 +1083,6 @@ __device__ __forceinline__ void put_group_sums(const SampleParams& p, double* to
 template <int DT>
 __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
   constexpr int EPL = Lane<DT, false>::EPL, IT = kChunk / (256 * EPL);
-  constexpr int kHeld = 1024;  // maxima at most
   __shared__ float bound, top;
   __shared__ double whole;
   __shared__ int count[2];
@@ -1093,7 +1095,7 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
   bool nucleus = s.k == 0 && s.p < 1.f;
   const bool minima = s.k == 0 && s.mp > 0.0;
   const ListRule rule = list_rule(s, p.groups);
-  const bool listing = rule.n > 0 && rule.n <= kHeld;
+  const bool listing = rule.n > 0;
   const int c0 = wg_id_x() * p.per, c1 = min(c0 + p.per, p.chunks);
   if (!listing && !nucleus && !minima) {
     if (c0 == 0 && tid == 0) p.low[row] = kNegInf;
@@ -1110,11 +1112,20 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams p) {
   if (wave == 0) {
     float b = kNegInf;
     if (listing) {
-      const float* gm =
-          rule.fine ? p.smax + (int64_t)row * p.groups * 4 : p.gmax + (int64_t)row * p.groups;
-      b = rule.n <= 128   ? list_bound<2>(gm, rule.n, rule.k)
-          : rule.n <= 256 ? list_bound<4>(gm, rule.n, rule.k)
-                          : list_bound<kHeld / 64>(gm, rule.n, rule.k);
+      const float* gm = p.gmax + (int64_t)row * p.groups;
+      const float* sm = p.smax + (int64_t)row * p.groups * 16;
+      auto quarter = [&](int g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(sm + 4 * g);
+        return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      };
+      if (rule.span == 16)
+        b = rule.n <= 128 ? list_bound<2>([&](int g) { return gm[g]; }, rule.n, rule.k)
+                          : list_bound<kHeld / 64>([&](int g) { return gm[g]; }, rule.n, rule.k);
+      else if (rule.span == 4)
+        b = rule.n <= 256 ? list_bound<4>(quarter, rule.n, rule.k)
+                          : list_bound<kHeld / 64>(quarter, rule.n, rule.k);
+      else
+        b = list_bound<kHeld / 64>([&](int g) { return sm[g]; }, rule.n, rule.k);
     }
     if (lane == 0) bound = b;
   } else if (wave == 1 && (nucleus || minima)) {
@@ -1632,17 +1643,17 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
 }
 
 // ---- small vocabularies ------------------------------------------------------------------------
-// A row in the registers of one workgroup, 8 logits a thread: one launch. top_k: the k-th largest of
+// A row in the registers of one workgroup, 8 or 16 logits a thread: one launch. top_k: the k-th largest of
 // the threads' maxima bounds the list, as in the gather; a nucleus: its histogram in LDS, then the
 // boundary's bins listed.
-constexpr int kSmall = 8 * kPick;
+constexpr int kSmall = 16 * kPick;
 static_assert(sizeof(PickShared::bin) >= kCutBins * 4 && sizeof(PickShared::bin) >= kPick * 4, "");
 
-template <int DT, bool TINY>
+template <int DT, bool TINY, int PER>
 __global__ __launch_bounds__(kPick) void sample_small_kernel(SampleParams p) {
   extern __shared__ __attribute__((aligned(16))) char pick_lds[];
   PickShared& sh = *reinterpret_cast<PickShared*>(pick_lds);
-  constexpr int PER = 8, EPL = Lane<DT, TINY>::EPL;
+  constexpr int EPL = Lane<DT, TINY>::EPL;
   const int rowi = wg_id_x(), tid = item_id(), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Row<DT, TINY> row;
@@ -1709,7 +1720,7 @@ __global__ __launch_bounds__(kPick) void sample_small_kernel(SampleParams p) {
       __syncthreads();
       const int n_top = (p.vocab + PER - 1) / PER;
       if (wave == 0) {
-        const float b = s.k <= n_top ? list_bound<kPick / 64>(top, n_top, s.k) : kNegInf;
+        const float b = s.k <= n_top ? list_bound<kPick / 64>([&](int g) { return top[g]; }, n_top, s.k) : kNegInf;
         if (lane == 0) sh.logz = (double)b;
       }
       __syncthreads();
@@ -1836,28 +1847,32 @@ hipError_t large_lds(K kernel) {
 }
 
 // (TINY: fewer tokens than a lane's load)
-template <int DT, bool TINY>
+template <int DT, bool TINY, int PER>
 hipError_t launch_small(const SampleParams& p, hipStream_t st) {
-  static const hipError_t once = large_lds(sample_small_kernel<DT, TINY>);
+  static const hipError_t once = large_lds(sample_small_kernel<DT, TINY, PER>);
   if (once != hipSuccess) return once;
-  hipLaunchKernelGGL((sample_small_kernel<DT, TINY>), dim3((unsigned)p.rows), dim3(kPick),
+  hipLaunchKernelGGL((sample_small_kernel<DT, TINY, PER>), dim3((unsigned)p.rows), dim3(kPick),
                      sizeof(PickShared), st, p);
   return hipGetLastError();
 }
 
 template <int DT>
 hipError_t launch_sample(const SampleParams& p, hipStream_t st) {
-  if (p.vocab < Lane<DT, false>::EPL) return launch_small<DT, true>(p, st);
-  if (p.vocab <= kSmall) return launch_small<DT, false>(p, st);
-  static const hipError_t once = large_lds(sample_pick_kernel<DT, true>);
-  if (once != hipSuccess) return once;
-  const unsigned rows = (unsigned)p.rows;
+  if (p.vocab < Lane<DT, false>::EPL) return launch_small<DT, true, 8>(p, st);
+  if (p.vocab <= kSmall / 2) return launch_small<DT, false, 8>(p, st);
   // what rows may do, as far as the host knows
   const bool counts = p.k || p.k_all > 0, nuclei = p.p || p.p_all < 1.f;
   const bool minima = p.mp || p.mp_all > 0.f, all_count = !p.k && p.k_all > 0 && p.k_all < p.vocab;
+  const bool filter = counts || nuclei || minima;
+  // (16 logits a thread: 113 x 10101 top-p 38 us, 52 in four launches; 31 x 8691 without a filter 14.5
+  // us, 12.9 in two)
+  if (p.vocab <= kSmall && filter) return launch_small<DT, false, 16>(p, st);
+  static const hipError_t once = large_lds(sample_pick_kernel<DT, true>);
+  if (once != hipSuccess) return once;
+  const unsigned rows = (unsigned)p.rows;
   hipLaunchKernelGGL(sample_scan_kernel<DT>, dim3((unsigned)((p.groups + 3) / 4), rows), dim3(256), 0,
                      st, p);
-  if (!counts && !nuclei && !minima) {
+  if (!filter) {
     hipLaunchKernelGGL((sample_pick_kernel<DT, false>), dim3(rows), dim3(kPick), sizeof(DrawShared), st,
                        p);
     return hipGetLastError();
@@ -1904,7 +1919,7 @@ SampleSpace sample_space(int32_t rows, int32_t vocab) {
   s.cand2 = take(c * kShort * 8);
   s.hist = take((size_t)rows * ((chunks + per - 1) / per) * kCutBins * 4);
   s.gmax = take(g * 4);
-  s.smax = take(g * 16);
+  s.smax = take(g * 64);
   s.low = take((size_t)rows * 4);
   s.count = take(c * 4);
   s.count2 = take(c * 4);

@@ -5,8 +5,9 @@
 // c = scale log2(e). Both sums may be cut anywhere: a piece over any set of keys is its own
 // (m, l = sum w, O = sum w v), and pieces join by 2^(m_piece - m) (prefix_merge_kernel).
 //
-// prefix_unit_kernel, one launch: a workgroup takes one piece of keys and up to 32 query rows
-// that read them. Prefix pieces come first (the rows of every slot and head of the group that
+// Few tiles: prefix_whole_kernel, whole slots in one launch (below). Otherwise
+// prefix_unit_kernel: a workgroup takes one piece of keys and up to 32 query rows that read them
+// (128 of the prefix's where there are many: prefix_rows). Prefix pieces come first (the rows of every slot and head of the group that
 // read one K/V head are the columns of one S^T = K Q^T product, so the prefix leaves HBM once per
 // 32 rows, and later row blocks find it in L2), then the slots' own pieces. Each of the four
 // waves takes 64-key tiles of its own, by DMA into its own LDS region, so all the workgroup's
@@ -329,9 +330,9 @@ struct PrefixWave {
     }
   }
 
-  // Whether every result so far is finite (AHEAD: its registers allow a second go). (A row that shares a tile with a non-finite V that it does
-  // not see is not: then the wave starts again, carefully. Results that are rightly non-finite come
-  // out the same from the second go.)
+  // Whether every result so far is finite (AHEAD: its registers allow a second go). A row that shares
+  // a tile with a non-finite V that it does not see is not: then the wave starts again, carefully.
+  // Results that are rightly non-finite come out the same from the second go.
   __device__ __forceinline__ bool finite() const {
     bool bad = false;
 #pragma unroll

@@ -44,8 +44,8 @@ extern "C" {
  * to their element.
  *
  * The workspace holds partial results only: it needs no clearing and is free again once the
- * call's work on `stream` is done; calls that may overlap need one each. 16-byte aligned. Results
- * are the same bits at every call. */
+ * call's work on `stream` is done; calls that may overlap need one each. 16-byte aligned. Short
+ * sequences need none (0 bytes; then it may be NULL). Results are the same bits at every call. */
 int ffai_prefix_attn_fwd(const ffai_kv_cache* prefix, const ffai_kv_cache* own, const void* q,
                          int32_t q_dtype, int32_t heads_q, int32_t q_len,
                          const int64_t* q_strides, float scale, void* out, int32_t out_dtype,

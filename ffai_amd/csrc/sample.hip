@@ -1007,8 +1007,10 @@ __device__ __forceinline__ float list_bound(F maximum, int n, int k) {
 #pragma unroll 1
   for (int step = 0; step < 20 && lo < hi; ++step) {
     const uint32_t mid = lo + (hi - lo) / 2 + 1;
-    if (at_least(mid) >= k) lo = mid;
+    const int c = at_least(mid);
+    if (c >= k) lo = mid;
     else hi = mid - 1;
+    if (c == k) break;
   }
   return of_key(lo);
 }
@@ -1361,13 +1363,19 @@ __device__ __forceinline__ bool cut_range(SH& sh, const CutBins& bins, const Row
   // the bins' ends by bisection: the least key of bins [0, lo - 1] (lanes 0 .. 31) and of [0, hi]
   uint32_t kx = key_of(kNegInf) + 1, ky = key_of(bins.m);
   const float b = (float)(lane < 32 ? lo : hi + 1);
-  while (__ballot(kx < ky)) {
-    const uint32_t mid = kx + (ky - kx) / 2;
-    if (kx < ky) {
-      if (bins.pos(of_key(mid)) < b) ky = mid;
-      else kx = mid + 1;
-    }
+  auto probe = [&](uint32_t k) {
+    if (bins.pos(of_key(k)) < b) ky = k;
+    else kx = k + 1;
+  };
+  // (the first two next to where the end must lie: a few steps then, 30 without)
+  const float far = b / bins.scale, near = far * 0x1p-20f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t k = key_of(bins.m - far + (j ? near : -near));
+    if (k >= kx && k < ky) probe(k);
   }
+  while (__ballot(kx < ky))
+    if (kx < ky) probe(kx + (ky - kx) / 2);
   const uint32_t k_lo = (uint32_t)__shfl((int)kx, 0), k_hi = (uint32_t)__shfl((int)kx, 32);
   *top = lo == 0 ? bins.m : of_key(k_lo - 1);
   *bottom = of_key(k_hi);
@@ -1760,7 +1768,7 @@ __global__ __launch_bounds__(kPick) void sample_small_kernel(SampleParams p) {
         token = pick_wide(row, sh, s, m, 0.0, u);
       }
     } else if (s.p < 1.f) {
-      double x = 0.0, y = 0.0, total;
+      double x = 0.0, y = 0.0;
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
         const double w = weight(v[e], m, s.inv2);

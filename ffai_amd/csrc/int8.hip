@@ -560,15 +560,25 @@ hipError_t launch_few_out(const Int8Params& p, int32_t y_dtype, const void* x, i
 struct Int8Tile {
   int bx, bw, waves, stages;
 };
-constexpr Int8Tile kTiles[] = {{256, 256, 8, 2}, {128, 128, 4, 2}, {64, 64, 4, 4}};
+constexpr Int8Tile kTiles[] = {{256, 256, 8, 2}, {128, 128, 8, 2}, {64, 64, 4, 4}};
 
+// The tile of least cost, in rounds of one 256^2 tile on each of the 256 CUs: two 128^2 tiles a CU take
+// 0.62 of that, two 64^2 ones 0.26 (24000 x 5120 x 1280: 145, 171 and 296 us), and one where a CU has no
+// second 0.6 of two. A larger tile within 5%, since it wins with the length of the contraction.
+// 1500 x 1280 x 3840: 128^2 16 us, 256^2 24, 64^2 25; 1500 x 1280 x 1280: 64^2 8.6, 128^2 9.4; 4000 x 1000 x
+// 6000: 128^2 42, 256^2 45; 3000 x 4000 x 3000: 256^2 54, 128^2 59.
 int int8_tile(int rows, int out_dim) {
-  for (int t = 0; t < 2; ++t) {
-    const int64_t n = (int64_t)((rows + kTiles[t].bx - 1) / kTiles[t].bx) *
-                      ((out_dim + kTiles[t].bw - 1) / kTiles[t].bw);
-    if (n >= 256) return t;
-  }
-  return 2;
+  auto tiles = [&](int t) {
+    return (int64_t)((rows + kTiles[t].bx - 1) / kTiles[t].bx) *
+           ((out_dim + kTiles[t].bw - 1) / kTiles[t].bw);
+  };
+  auto pairs = [&](int t, double two) {
+    const int64_t n = tiles(t), rest = n % 512;
+    return two * ((double)(n / 512) + (rest == 0 ? 0.0 : rest <= 256 ? 0.6 : 1.0));
+  };
+  const double large = (double)((tiles(0) + 255) / 256), middle = pairs(1, 0.62), small = pairs(2, 0.26);
+  if (large <= 1.05 * std::min(middle, small)) return 0;
+  return middle <= 1.05 * small ? 1 : 2;
 }
 
 template <int BX, int BW, int GX, int GW, int STAGES, int OCC, int OUT>
@@ -588,7 +598,7 @@ hipError_t launch_product(Int8Params p, hipStream_t st) {
   p.tx = (p.rows + kTiles[t].bx - 1) / kTiles[t].bx;
   p.tw = (p.out_dim + kTiles[t].bw - 1) / kTiles[t].bw;
   if (t == 0) return launch_tile<256, 256, 2, 4, 2, 2, OUT>(p, st);
-  if (t == 1) return launch_tile<128, 128, 2, 2, 2, 2, OUT>(p, st);
+  if (t == 1) return launch_tile<128, 128, 2, 4, 2, 4, OUT>(p, st);
   return launch_tile<64, 64, 2, 2, 4, 2, OUT>(p, st);
 }
 

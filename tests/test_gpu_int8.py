@@ -262,3 +262,50 @@ def test_tiles_cover_the_grid():
     for m, k, n in SIZES + [(24000, 5120, 1280), (1500, 1280, 3840)]:
         p = plan_info(m, k, n)
         assert p["workgroups"] >= -(-m // p["tile_rows"]) * -(-n // p["tile_outputs"])
+
+
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m,k,n,tile", [(3900, 200, 4010, 256), (2500, 130, 1030, 128),
+                                        (600, 300, 1030, 64)])
+def test_every_tile_into_every_type(gpu, m, k, n, tile, out):
+    """Ragged on both sides, y with rows of a larger buffer whose other elements stay."""
+    assert plan_info(m, k, n)["tile_rows"] == tile
+    t = rand(gpu, m, k, seed=8, dtype=torch.float16)
+    lin, w, sw, b = layer(gpu, n, k, True)
+    y = torch.full((m, n + 5), 7.0, dtype=DT[out], device=gpu)
+    lin(t, out=y[:, 3:3 + n])
+    q, s = oracle8.quantize_rows(t.float().cpu().numpy())
+    same(y[:, 3:3 + n], oracle8.linear(q, s, w, sw, b), True)
+    assert (y[:, :3] == 7).all() and (y[:, 3 + n:] == 7).all()
+
+
+def test_many_rows_past_32_bit_offsets(gpu):
+    m, k, n, stride = 20, 256, 64, 1 << 27
+    x = torch.empty(m, stride, dtype=torch.float16, device=gpu)[:, :k]
+    x.copy_(rand(gpu, m, k, seed=16))
+    y = torch.empty(m, stride + 64, dtype=torch.float16, device=gpu)[:, :n]
+    lin, w, sw, b = layer(gpu, n, k, True)
+    lin(x, out=y)
+    q, s = oracle8.quantize_rows(x.float().cpu().numpy())
+    same(y, oracle8.linear(q, s, w, sw, b), True)
+
+
+def test_few_rows_on_streams_and_in_graphs(gpu):
+    lin, w, sw, b = layer(gpu, 130, 2300, True)
+    x = rand(gpu, 7, 2300, seed=17)
+    first = lin(x)
+    torch.cuda.synchronize()
+    outs = []
+    for s in [torch.cuda.Stream() for _ in range(2)] * 3:
+        with torch.cuda.stream(s):
+            outs.append(lin(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, o) for o in outs)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = lin(x)
+    for i in range(3):
+        x.copy_(torch.randn_like(x))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, lin(x))

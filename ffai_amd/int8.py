@@ -90,6 +90,7 @@ class Int8Linear:
         self.out_dim, self.in_dim = qw.shape[0], in_dim
         self._w = (qw.data_ptr(), qw.stride(0), scale.data_ptr(),
                    None if bias is None else bias.data_ptr(), self.out_dim)
+        self._sized = (0, 0)  # the last number of rows, and its workspace
         self._few = 0  # up to so many rows need no workspace
         while self._few < 64 and self.workspace_bytes(self._few + 1) == 0:
             self._few += 1
@@ -134,7 +135,10 @@ class Int8Linear:
                 raise ValueError(f"workspace must be contiguous, on {device}")
             work, n = workspace.data_ptr(), workspace.nbytes
         elif rows > self._few:
-            n = self.workspace_bytes(rows)
+            sized = self._sized
+            if sized[0] != rows:
+                sized = self._sized = (rows, self.workspace_bytes(rows))
+            n = sized[1]
             workspace = torch.empty(n, dtype=torch.uint8, device=device)
             work = workspace.data_ptr()
         L.call_on(device, L.load().ffai_int8_linear, x2.data_ptr(), _DT[x2.dtype], x2.stride(0), rows,

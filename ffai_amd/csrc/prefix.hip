@@ -183,13 +183,15 @@ PrefixPlan plan_prefix(const ffai_kv_cache* pre, const ffai_kv_cache* own, int h
   const int64_t units_p = units * p.blocks_p;
   // Key pieces: enough workgroups for two on every CU, but no fewer than four tiles (one a wave)
   // to a piece, since every piece of a row is written once and read once by the merge. Blocks of
-  // 128 rows: one workgroup on every CU beside the own pieces, eight tiles at least.
+  // 128 rows: one workgroup on every CU, which leaves its other place to the own pieces' stream under
+  // those products, eight tiles at least (128 slots x 32 heads, 16384 shared and 33 to 1024 own keys: 95
+  // us; two workgroups on every CU, twice the pieces, 113; one and a half 103).
   constexpr int64_t kTarget = 512;
   auto pieces = [&](int64_t tiles, int64_t least, int64_t target, int64_t n) {
     return (int)std::min<int64_t>(std::min<int64_t>(ceil_div(tiles, least), 64),
                                   std::max<int64_t>(1, ceil_div(target, n)));
   };
-  p.pieces_p = p.many ? pieces(tiles_p, 8, kTarget, units_p)
+  p.pieces_p = p.many ? pieces(tiles_p, 8, kTarget / 2, units_p)
                       : pieces(tiles_p, 4, std::max<int64_t>(kTarget - units_o, kTarget / 2), units_p);
   p.pieces_o = pieces(tiles_o, 4, kTarget - (p.many ? 0 : units_p * p.pieces_p), units_o);
   p.items_p = units_p * p.pieces_p;

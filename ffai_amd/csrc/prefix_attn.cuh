@@ -769,8 +769,9 @@ __device__ __forceinline__ void prefix_rows(const PrefixParams& p, const PrefixW
 }
 
 // ROWS: the prefix's pieces run as prefix_rows (many rows), else as prefix_work in blocks of 16 NCP
-// rows; the own pieces always as prefix_work. The prefix's come first in the grid: 128 slots x 32
-// heads, 16384 shared and 33 to 1024 own keys 107 us, with the two kinds in turn 109 to 119.
+// rows; the own pieces always as prefix_work. The prefix's come first in the grid, one a CU where they
+// are prefix_rows: the own ones then stream beside them. 128 slots x 32 heads, 16384 shared and 33 to
+// 1024 own keys 95 us, of which the merge 6.
 template <int DT, int D, int NQ, int NP, int NCP, int NCO, bool ROWS>
 __global__ __launch_bounds__(kPrefixWaves * 64, NQ > 1 && (NCP > 1 || NCO > 1 || D == 128) ? 1 : 2) void
 prefix_unit_kernel(PrefixParams p) {

@@ -92,7 +92,7 @@ struct RowScale {
   float s, inv;
   bool fast;
   __device__ __forceinline__ RowScale(uint32_t top) {
-    s = top == 0 ? 1.f : __uint_as_float(top) / 127.f;
+    s = top == 0 ? 1.f : __uint_as_float(top) * (1.f / 127.f);
     inv = 1.f / s;
     fast = finite_bits(s) && finite_bits(inv);
   }

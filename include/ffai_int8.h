@@ -7,7 +7,8 @@
  * take any number of rows: a prompt's tokens, a batch of sequences, an encoder's frames. No
  * counterpart in the reference.
  *
- *   s[m] = max_k |x[m][k]| / 127 (1 where the row is all zero), an f32 quotient
+ *   s[m] = max_k |x[m][k]| * (1 / 127) in f32, both factors f32 (1 where the row is all zero): what
+ *          `amax / 127` gives where a division by a constant is that product, as on this device
  *   q[m][k] = round-half-even(x[m][k] / s[m]), of the f32 quotient, in [-127, 127]
  *   acc[m][n] = sum_k q[m][k] * w[n][k], exact in 32-bit integers (in_dim <= 131072)
  *   y[m][n] = (f32(acc) * s[m]) * w_scale[n] + bias[n] in f32 (the last product and the sum

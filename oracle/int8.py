@@ -1,5 +1,6 @@
 """Linear layers in 8-bit integers, restated in numpy from the definition: the check for
-ffai_amd.int8. Quotients are IEEE f32, sums exact integers, the rest in f32 step by step."""
+ffai_amd.int8. Scales are the largest magnitude times the f32 number nearest to 1 / 127, quotients
+IEEE f32, sums exact integers, the rest in f32 step by step."""
 
 from __future__ import annotations
 
@@ -11,7 +12,7 @@ def quantize_rows(x):
     x = np.asarray(x, np.float32)
     top = np.abs(x).max(axis=1) if x.shape[1] else np.zeros(len(x), np.float32)
     with np.errstate(all="ignore"):
-        s = np.where(top == 0, np.float32(1), top / np.float32(127)).astype(np.float32)
+        s = np.where(top == 0, np.float32(1), top * (np.float32(1) / np.float32(127))).astype(np.float32)
         r = np.rint(x / s[:, None])  # numpy's rint rounds halves to even
         q = np.where(np.isnan(r), 0, np.clip(r, -127, 127)).astype(np.int8)
     return q, s

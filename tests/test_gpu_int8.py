@@ -93,7 +93,7 @@ def test_quotients_next_to_a_half(gpu, rows, dim):
     off: which integer each goes to is the division's."""
     g = np.random.default_rng(dim)
     top = np.float32(1) + g.random((rows, 1), dtype=np.float32)
-    s = top / np.float32(127)
+    s = top * (np.float32(1) / np.float32(127))
     half = g.integers(-127, 127, (rows, dim)).astype(np.float32) + np.float32(0.5)
     x = (half * s).astype(np.float32)
     ulps = g.integers(-3, 4, (rows, dim)).astype(np.int32)
@@ -309,3 +309,12 @@ def test_few_rows_on_streams_and_in_graphs(gpu):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, lin(x))
+
+
+def test_scales_are_the_devices_amax_over_127(gpu):
+    """Weights quantized by elementary device operations have the same scales and integers."""
+    w = rand(gpu, 3000, 700, seed=23)
+    qr = quantize_rows(w)
+    s = w.abs().amax(1) / 127
+    assert torch.equal(qr.scale, s)
+    assert torch.equal(qr.q[:, :700].float(), torch.round(w / s[:, None]))

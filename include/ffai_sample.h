@@ -19,7 +19,7 @@
  * off. A row without a finite or infinite maximum (all -inf or NaN) gives token -1.
  * logprob: log softmax(l)[token] at temperature 1 over the whole row, -inf for token -1.
  *
- * Token choices are exact to 64-bit rounding (about 1e-13 of the row's weight) and the same at
+ * Token choices are exact to 64-bit rounding (below 1e-12 of the row's weight) and the same at
  * every call. All calls are asynchronous on `stream` (a hipStream_t; NULL = null stream), allocate
  * nothing, take device pointers of the current device and return FFAI_OK or a negative
  * ffai_status (ffai_attn.h), with the reason in ffai_attn_last_error().
